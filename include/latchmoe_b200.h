@@ -45,6 +45,10 @@ extern "C" {
 #define LM_DEVERR_UNMAPPED_EXPERT 2 /* expert routed but its group/slot entry is -1 */
 #define LM_DEVERR_WAIT_TIMEOUT 3    /* a bounded mbarrier wait gave up */
 #define LM_DEVERR_BAD_GROUP 4       /* group table inconsistent with the pair table */
+#define LM_DEVERR_NO_PAGES 5        /* no free cache page, or a full block-table row */
+#define LM_DEVERR_BAD_LENGTH 6      /* a length, count or token offset outside its buffer */
+#define LM_DEVERR_BAD_PAGE 7        /* block-table entry or slot outside the cache */
+#define LM_DEVERR_BAD_POSITION 8    /* position outside the rotary table */
 
 /* Scoring functions accepted by lm_route_topk (reference `scoring_func`). */
 #define LM_SCORING_SOFTMAX 0
@@ -470,6 +474,102 @@ int lm_ep_combine(const int32_t* topk_ids, const uint16_t* topk_weights_bf16,
                   const int32_t* send_offsets, int32_t rank, int32_t world,
                   void* const* peer_regions, void* local_region, int32_t cap, int64_t epoch,
                   uint16_t* out, int32_t* err_word, void* stream);
+
+/* ---------------------------------------------------------------------------------------
+ * The attention half of a decoder layer around the MoE layer: norm, rotary embedding, paged KV
+ * cache and attention. (The reference leaves these to the vLLM fork that it plugs into.)
+ *
+ * Paged cache: K and V are [num_pages][page_size][kv heads][head_dim] bf16 with free page, token
+ * and head strides (elements); head_dim values are contiguous. A request's row of the block table
+ * names its pages in order; slot = page * page_size + offset, -1 for a token without a place.
+ * Lengths and tables live on the device and are read there, so a captured call serves any batch
+ * of its size. All of these are launched with programmatic stream serialisation.
+ */
+
+/* Residual addition and RMS norm: z = x + residual (fp32); residual_out = bf16(z);
+ * y = z * rsqrt(mean(z^2) + eps) * weight, rounded once to bf16 (y) or to e4m3 (y8, with fp32
+ * scales: s = max(max|y|, 1e-12) / 448 per row (group_size 0, scales [T]) or per group_size
+ * columns (a multiple of 32 that divides hidden_size; scales [T][hidden_size / group_size]);
+ * y8 = e4m3(y / s)). Exactly one of y and y8. residual and residual_out may be NULL;
+ * residual_out may be residual or x itself (with the same stride), other overlaps may not.
+ * Strides are row strides in elements; hidden_size <= 16384. */
+int lm_add_rms_norm(const uint16_t* x, int64_t x_stride, const uint16_t* residual,
+                    int64_t residual_stride, const uint16_t* weight, float eps,
+                    int64_t num_tokens, int32_t hidden_size, uint16_t* residual_out,
+                    int64_t residual_out_stride, uint16_t* y, int64_t y_stride, uint8_t* y8,
+                    int64_t y8_stride, float* scales, int32_t group_size, void* stream);
+
+/* Tables of one step for num_requests (<= 4096) rows with cached_lens[b] tokens in the cache and
+ * new_lens[b] new ones (0: an idle row). Row b of block_tables holds ceil(cached / page_size)
+ * pages already; the pages that its new tokens need are granted in row order from the end of the
+ * free stack (free_pages[0 .. *free_count)) and written behind them.
+ *   seq_lens[b] = cached + new;  cu_q[0 .. num_requests] = exclusive sums of new_lens;
+ *   positions[t], slot_mapping[t] for the new tokens in row order; past the last one, up to
+ *   max_tokens, position 0 and slot -1;  *free_count_out = what is left on the stack.
+ * free_count_out may be free_count and seq_lens may be cached_lens (the step's state, in place);
+ * a call with other outputs changes nothing that it reads, so it may be repeated.
+ * A row without enough free pages or table columns gets none (LM_DEVERR_NO_PAGES): its tokens have
+ * slot -1 and its sequence length stays; so do all rows behind it that need a page, if the stack
+ * ran out. A bad length counts as 0 (LM_DEVERR_BAD_LENGTH), tokens past max_tokens are cut. */
+int lm_build_page_tables(const int32_t* cached_lens, const int32_t* new_lens,
+                         int32_t num_requests, int32_t page_size, int32_t* block_tables,
+                         int64_t table_stride, int32_t max_pages, const int32_t* free_pages,
+                         int32_t free_capacity, const int32_t* free_count,
+                         int32_t* free_count_out, int32_t* seq_lens, int32_t* cu_q,
+                         int32_t* positions, int64_t* slot_mapping, int64_t max_tokens,
+                         int32_t* err_word, void* stream);
+
+/* The pages of the listed rows (ceil(cached_lens / page_size) entries each) go back onto the free
+ * stack in the order of the list; their table entries become -1 and their lengths 0. A row outside
+ * the table or a stack overflow is recorded (LM_DEVERR_BAD_LENGTH) and skipped. */
+int lm_release_pages(const int32_t* rows, int32_t num_rows, int32_t* cached_lens,
+                     int32_t num_requests, int32_t page_size, int32_t* block_tables,
+                     int64_t table_stride, int32_t max_pages, int32_t* free_pages,
+                     int32_t free_capacity, int32_t* free_count, int32_t* err_word, void* stream);
+
+/* qkv [T][(q heads + 2 kv heads) * head_dim] (row stride qkv_stride): q and k heads get the
+ * optional RMS norm over head_dim (weights [head_dim], or NULL) and the rotary embedding of their
+ * first rot_dim values (pairs (i, i + rot_dim / 2), or neighbours when interleaved;
+ * cos_sin [max_positions][rot_dim] fp32: cosines, then sines). q goes to q_out, k and v to
+ * slot_mapping[t] of the cache; a slot of -1 stores no k and v. fp32 inside, one rounding.
+ * q_out may be the q part of qkv. head_dim 64 or 128; bases 16-byte aligned, strides multiples of
+ * 8 elements. A slot past the cache (LM_DEVERR_BAD_PAGE) is not stored; a position outside the
+ * table (LM_DEVERR_BAD_POSITION) counts as 0. */
+int lm_rope_cache_write(const uint16_t* qkv, int64_t qkv_stride, const int32_t* positions,
+                        const int64_t* slot_mapping, int64_t num_tokens, int32_t num_q_heads,
+                        int32_t num_kv_heads, int32_t head_dim, const float* cos_sin,
+                        int32_t max_positions, int32_t rot_dim, int32_t interleaved,
+                        const uint16_t* q_norm_weight, const uint16_t* k_norm_weight, float eps,
+                        uint16_t* q_out, int64_t q_token_stride, int64_t q_head_stride,
+                        uint16_t* k_cache, int64_t k_page_stride, int64_t k_token_stride,
+                        int64_t k_head_stride, uint16_t* v_cache, int64_t v_page_stride,
+                        int64_t v_token_stride, int64_t v_head_stride, int64_t num_pages,
+                        int32_t page_size, int32_t* err_word, void* stream);
+
+/* Attention of the step's tokens over the cache: request b's queries are tokens
+ * cu_q[b] .. cu_q[b + 1] and the last of them stands at position seq_lens[b] - 1. A query at
+ * position p sees key j when j <= p and (window == 0 or j > p - window). out [T][q heads]
+ * [head_dim] bf16; lse [T][q heads] fp32 (may be NULL) = ln of the sum of exp(scale * q.k). A query
+ * that sees no key gives zeros and an lse of -inf; tokens of no request are not written. Keys that
+ * no query of a row tile sees are not read (stale cache contents, NaN included, do not matter).
+ * head_dim 64 or 128, page_size a multiple of 16, num_q_heads a multiple of num_kv_heads, at most
+ * 4096 requests; bases 16-byte aligned, strides multiples of 8 elements. max_q_len only chooses
+ * kernels; results do not depend on it being right. The workspace
+ * (lm_paged_attention_workspace_bytes() for the current device, 16-byte aligned, zeroed once) is
+ * left ready for the next call; calls that share one must not overlap. A table entry outside the
+ * cache is recorded (LM_DEVERR_BAD_PAGE) and its keys count as zeros. */
+int64_t lm_paged_attention_workspace_bytes(void);
+int lm_paged_attention(const uint16_t* q, int64_t q_token_stride, int64_t q_head_stride,
+                       const uint16_t* k_cache, int64_t k_page_stride, int64_t k_token_stride,
+                       int64_t k_head_stride, const uint16_t* v_cache, int64_t v_page_stride,
+                       int64_t v_token_stride, int64_t v_head_stride, int64_t num_pages,
+                       int32_t page_size, const int32_t* block_tables, int64_t table_stride,
+                       int32_t max_pages, const int32_t* seq_lens, const int32_t* cu_q,
+                       int32_t num_requests, int64_t num_tokens, int32_t num_q_heads,
+                       int32_t num_kv_heads, int32_t head_dim, int32_t max_q_len, float scale,
+                       int32_t window, uint16_t* out, int64_t out_token_stride,
+                       int64_t out_head_stride, float* lse, void* workspace,
+                       int64_t workspace_bytes, int32_t* err_word, void* stream);
 
 #ifdef __cplusplus
 }

@@ -28,6 +28,10 @@ DEVERR_NAMES = {
     2: "expert routed but unmapped (log2phy/group entry is -1)",
     3: "bounded device wait timed out",
     4: "group table inconsistent with the pair table",
+    5: "no free cache page, or a full block-table row",
+    6: "length, count or token offset outside its buffer",
+    7: "block-table entry or slot outside the cache",
+    8: "position outside the rotary table",
 }
 
 # Every symbol include/latchmoe_b200.h declares, with (restype, argtypes).
@@ -131,6 +135,28 @@ SIGNATURES: dict[str, tuple[object, list[object]]] = {
     "lm_stage_copy": (
         ctypes.c_int,
         [_P, _I64, _P, _I64, _P, _P, _I32, _I64, _I32, _P],
+    ),
+    "lm_add_rms_norm": (
+        ctypes.c_int,
+        [_P, _I64, _P, _I64, _P, _F32, _I64, _I32, _P, _I64, _P, _I64, _P, _I64, _P, _I32, _P],
+    ),
+    "lm_build_page_tables": (
+        ctypes.c_int,
+        [_P, _P, _I32, _I32, _P, _I64, _I32, _P, _I32, _P, _P, _P, _P, _P, _P, _I64, _P, _P],
+    ),
+    "lm_release_pages": (
+        ctypes.c_int, [_P, _I32, _P, _I32, _I32, _P, _I64, _I32, _P, _I32, _P, _P, _P]),
+    "lm_rope_cache_write": (
+        ctypes.c_int,
+        [_P, _I64, _P, _P, _I64, _I32, _I32, _I32, _P, _I32, _I32, _I32, _P, _P, _F32, _P, _I64,
+         _I64, _P, _I64, _I64, _I64, _P, _I64, _I64, _I64, _I64, _I32, _P, _P],
+    ),
+    "lm_paged_attention_workspace_bytes": (ctypes.c_int64, []),
+    "lm_paged_attention": (
+        ctypes.c_int,
+        [_P, _I64, _I64, _P, _I64, _I64, _I64, _P, _I64, _I64, _I64, _I64, _I32, _P, _I64, _I32,
+         _P, _P, _I32, _I64, _I32, _I32, _I32, _I32, _F32, _I32, _P, _I64, _I64, _P, _P, _I64, _P,
+         _P],
     ),
 }
 

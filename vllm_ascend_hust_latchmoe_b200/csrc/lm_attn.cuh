@@ -1,0 +1,171 @@
+// What the two attention kernels over the paged cache share: their parameters, the split of the
+// work over the CTAs, and the merge of partial results.
+//
+// Rows: a request's queries of one kv head are flattened to (token, query head of the group)
+// rows, so a row tile fills up whatever the number of query heads per kv head. An item is
+// (request, kv head, row tile); its cost is the number of kv blocks that its rows see. All items'
+// blocks are laid end to end and every CTA takes the same number of them, wherever that cuts an
+// item ("per" units each): the load is even whatever the requests' lengths, and one long sequence
+// spreads over the whole GPU. A CTA leaves at most two partial results: one of the item that it
+// continues and one of the item that it starts and does not finish.
+#pragma once
+
+#include "lm_common.cuh"
+
+namespace lm {
+
+constexpr int kAttnMaxRequests = 4096;
+constexpr int kAttnMaxCtas = 512;      // counters in the workspace
+constexpr int kAttnMaxPartialRows = 256;
+
+struct AttnParams {
+  const uint16_t* q;
+  const uint16_t* k;
+  const uint16_t* v;
+  uint16_t* out;
+  float* lse;  // [T, Hq] or null
+  const int32_t* tables;
+  const int32_t* seq_lens;
+  const int32_t* cu_q;
+  int32_t* counters;   // [kAttnMaxCtas], zero between launches
+  float* partial_o;    // [2 * ctas][rows][D]
+  float* partial_ml;   // [2 * ctas][rows][2]: running maximum (log2 domain) and sum
+  int32_t* err;
+  int64_t q_token_stride, q_head_stride, out_token_stride, out_head_stride;
+  int64_t k_page_stride, k_token_stride, k_head_stride;
+  int64_t v_page_stride, v_token_stride, v_head_stride;
+  int64_t table_stride;
+  int64_t num_tokens;
+  int num_requests, q_heads, kv_heads, group, page_size, num_pages, max_pages, window;
+  int min_rows, max_rows;  // requests with this many rows per kv head are this launch's
+  float scale_log2;        // softmax scale * log2(e)
+};
+
+struct AttnRequest {
+  int q0, qlen, seq;
+};
+
+// The request's query range and length, held inside their buffers.
+__device__ __forceinline__ AttnRequest attn_request(const AttnParams& p, int b, bool report) {
+  AttnRequest r;
+  r.q0 = p.cu_q[b];
+  const int q1 = p.cu_q[b + 1];
+  r.qlen = q1 - r.q0;
+  r.seq = p.seq_lens[b];
+  if (r.q0 < 0 || q1 < r.q0 || q1 > p.num_tokens) {
+    if (report) record_error(p.err, LM_DEVERR_BAD_LENGTH);
+    r.q0 = r.qlen = 0;
+  }
+  const int64_t limit = static_cast<int64_t>(p.max_pages) * p.page_size;
+  if (r.seq < 0 || r.seq > limit) {
+    if (report) record_error(p.err, LM_DEVERR_BAD_LENGTH);
+    r.seq = r.seq < 0 ? 0 : static_cast<int>(limit);
+  }
+  return r;
+}
+
+// Keys that some row of tile `tile` sees: [lo, hi).
+template <int TILE_ROWS>
+__device__ __forceinline__ void attn_tile_keys(const AttnParams& p, const AttnRequest& r, int tile,
+                                               int& lo, int& hi) {
+  const int rows = r.qlen * p.group;
+  const int first = tile * TILE_ROWS / p.group;
+  const int last = (min((tile + 1) * TILE_ROWS, rows) - 1) / p.group;
+  const int cached = r.seq - r.qlen;  // negative: the first queries stand before every key
+  hi = max(0, cached + last + 1);
+  lo = p.window > 0 ? min(hi, max(0, cached + first - p.window + 1)) : 0;
+}
+
+template <int BLOCK>
+__device__ __forceinline__ int attn_blocks(int lo, int hi) {
+  // an item without keys still costs a unit: its rows have to be written
+  return hi > lo ? (hi + BLOCK - 1) / BLOCK - lo / BLOCK : 1;
+}
+
+// Exclusive prefix of the requests' costs in s_prefix[0 .. B]. Called by all NT threads.
+template <int TILE_ROWS, int BLOCK, int NT>
+__device__ __forceinline__ void attn_prefix(const AttnParams& p, int32_t* s_prefix, int32_t* s_warp) {
+  const int B = p.num_requests;
+  const int per = (B + NT - 1) / NT;
+  const int b0 = threadIdx.x * per, b1 = min(B, b0 + per);
+  int sum = 0;
+  for (int b = b0; b < b1; ++b) {
+    const AttnRequest r = attn_request(p, b, blockIdx.x == 0);
+    const int rows = r.qlen * p.group;
+    int cost = 0;
+    if (rows >= p.min_rows && rows <= p.max_rows) {
+      const int tiles = (rows + TILE_ROWS - 1) / TILE_ROWS;
+      for (int t = 0; t < tiles; ++t) {
+        int lo, hi;
+        attn_tile_keys<TILE_ROWS>(p, r, t, lo, hi);
+        cost += attn_blocks<BLOCK>(lo, hi);
+      }
+    }
+    s_prefix[b + 1] = cost * p.kv_heads;
+    sum += cost * p.kv_heads;
+  }
+  int incl = sum;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const int u = __shfl_up_sync(0xffffffffu, incl, o);
+    if (lane >= o) incl += u;
+  }
+  if (lane == 31) s_warp[warp] = incl;
+  __syncthreads();
+  int base = incl - sum;
+  for (int w = 0; w < warp; ++w) base += s_warp[w];
+  for (int b = b0; b < b1; ++b) {
+    base += s_prefix[b + 1];
+    s_prefix[b + 1] = base;
+  }
+  if (threadIdx.x == 0) s_prefix[0] = 0;
+  __syncthreads();
+}
+
+// A CTA's piece of an item: kv blocks [blk0, blk1) of those that hold keys [lo, hi).
+struct AttnSegment {
+  AttnRequest req;
+  int b, head, tile;
+  int lo, hi;      // keys of the whole tile
+  int blk0, blk1;  // absolute kv block numbers of this segment
+  int start, end;  // the item's units [start, end) in the launch's order
+  bool whole;
+};
+
+// The segment at unit w of a CTA whose units end at w_end; every thread computes it alike.
+template <int TILE_ROWS, int BLOCK>
+__device__ __forceinline__ AttnSegment attn_segment(const AttnParams& p, const int32_t* s_prefix,
+                                                    int w, int w_end) {
+  int lo_b = 0, hi_b = p.num_requests;
+  while (hi_b - lo_b > 1) {  // the last request that starts at or before w; costless ones end there
+    const int mid = (lo_b + hi_b) >> 1;
+    if (s_prefix[mid] <= w) lo_b = mid; else hi_b = mid;
+  }
+  AttnSegment s;
+  s.b = lo_b;
+  s.req = attn_request(p, lo_b, false);
+  int off = w - s_prefix[lo_b];
+  const int per_head = (s_prefix[lo_b + 1] - s_prefix[lo_b]) / p.kv_heads;
+  s.head = off / per_head;
+  off -= s.head * per_head;
+  s.tile = 0;
+  int n;
+  for (;;) {
+    attn_tile_keys<TILE_ROWS>(p, s.req, s.tile, s.lo, s.hi);
+    n = attn_blocks<BLOCK>(s.lo, s.hi);
+    if (off < n) break;
+    off -= n;
+    ++s.tile;
+  }
+  s.start = w - off;
+  s.end = s.start + n;
+  const int u1 = min(n, off + w_end - w);
+  s.whole = off == 0 && u1 == n;
+  const int first = s.lo / BLOCK;
+  s.blk0 = first + off;
+  s.blk1 = s.hi > s.lo ? first + u1 : s.blk0;
+  return s;
+}
+
+}  // namespace lm
