@@ -79,19 +79,21 @@ __global__ void __launch_bounds__(kThreads, 1) paged_attn_rows_kernel(const Attn
   const int per = (total + gridDim.x - 1) / gridDim.x;
   int w = blockIdx.x * per;
   const int w_end = min(total, w + per);
+  AttnCursor at{};
+  if (w < w_end) at = attn_seek<kTileRows, kBlock>(p, s_prefix, w);
 
   unsigned char* ring = smem + warp * kStages * S::kStage;
   const uint32_t ring_addr = smem_u32(ring);
 
   while (w < w_end) {
-    const AttnSegment s = attn_segment<kTileRows, kBlock>(p, s_prefix, w, w_end);
-    const int rows = s.req.qlen * p.group;
-    const int row_base = s.tile * kTileRows;
-    const int cached = s.req.seq - s.req.qlen;
+    const AttnSegment s = attn_segment<kTileRows, kBlock>(p, at, w, w_end);
+    const int rows = at.req.qlen * p.group;
+    const int row_base = at.tile * kTileRows;
+    const int cached = at.req.seq - at.req.qlen;
     const int n_slices = s.blk1 - s.blk0;  // one slice of this warp per block
-    const int32_t* table = p.tables + s.b * p.table_stride;
-    const uint16_t* kh = p.k + s.head * p.k_head_stride;
-    const uint16_t* vh = p.v + s.head * p.v_head_stride;
+    const int32_t* table = p.tables + at.b * p.table_stride;
+    const uint16_t* kh = p.k + at.head * p.k_head_stride;
+    const uint16_t* vh = p.v + at.head * p.v_head_stride;
     int pages = 0, page_first = 0;  // lane i: the page of slice page_first + i
 
     auto load = [&](int i) {  // slice i of this warp into stage i % kStages
@@ -138,10 +140,10 @@ __global__ void __launch_bounds__(kThreads, 1) paged_attn_rows_kernel(const Attn
     uint32_t qf[D / 16][4];
     {
       const bool ok0 = r0 < rows, ok1 = r1 < rows;
-      const uint16_t* q0 = p.q + (s.req.q0 + t0) * p.q_token_stride +
-                           (s.head * p.group + r0 % p.group) * p.q_head_stride;
-      const uint16_t* q1 = p.q + (s.req.q0 + t1) * p.q_token_stride +
-                           (s.head * p.group + r1 % p.group) * p.q_head_stride;
+      const uint16_t* q0 = p.q + (at.req.q0 + t0) * p.q_token_stride +
+                           (at.head * p.group + r0 % p.group) * p.q_head_stride;
+      const uint16_t* q1 = p.q + (at.req.q0 + t1) * p.q_token_stride +
+                           (at.head * p.group + r1 % p.group) * p.q_head_stride;
 #pragma unroll
       for (int k = 0; k < D / 16; ++k) {
         qf[k][0] = ok0 ? *reinterpret_cast<const uint32_t*>(q0 + k * 16 + c2) : 0u;
@@ -312,9 +314,9 @@ __global__ void __launch_bounds__(kThreads, 1) paged_attn_rows_kernel(const Attn
       }
     }
     if (final && row_base + r < rows) {
-      const int tok = s.req.q0 + (row_base + r) / p.group;
-      const int head = s.head * p.group + (row_base + r) % p.group;
-      const float inv = l > 0.f ? 1.f / l : 0.f;
+      const int tok = at.req.q0 + (row_base + r) / p.group;
+      const int head = at.head * p.group + (row_base + r) % p.group;
+      const float inv = l != 0.f ? 1.f / l : 0.f;
       uint16_t* dst = p.out + tok * p.out_token_stride + head * p.out_head_stride + col;
       uint32_t packed[D / 32];
 #pragma unroll
@@ -325,9 +327,10 @@ __global__ void __launch_bounds__(kThreads, 1) paged_attn_rows_kernel(const Attn
         *reinterpret_cast<uint2*>(dst) = make_uint2(packed[0], packed[1]);
       if (p.lse != nullptr && (threadIdx.x & 15) == 0)
         p.lse[static_cast<int64_t>(tok) * p.q_heads + head] =
-            l > 0.f ? (m + log2f(l)) * 0.693147180559945309f : -INFINITY;
+            l != 0.f ? (m + log2f(l)) * 0.693147180559945309f : -INFINITY;
     }
-    w += s.blk1 > s.blk0 ? s.blk1 - s.blk0 : 1;
+    w += s.units;
+    if (w < w_end) attn_advance<kTileRows>(p, at);
     __syncthreads();  // the merge area is free for the next segment's loads
   }
 }
@@ -346,7 +349,7 @@ int attn_ctas() {
 
 // The workspace: counters, then the partial sums and accumulators of 2 partials per CTA.
 struct Workspace {
-  static constexpr int64_t kCounterBytes = kAttnMaxCtas * 4;
+  static constexpr int64_t kCounterBytes = 2 * kAttnMaxCtas * 4;
   static int64_t ml_bytes() { return static_cast<int64_t>(2) * attn_ctas() * kAttnMaxPartialRows * 8; }
   static int64_t o_bytes() {
     return static_cast<int64_t>(2) * attn_ctas() * kAttnMaxPartialRows * 128 * 4;
@@ -455,5 +458,16 @@ extern "C" int lm_paged_attention(
   p.min_rows = 1;
   p.max_rows = 0x7fffffff;
   cudaStream_t s = static_cast<cudaStream_t>(stream);
+  // Requests of up to 16 rows per kv head read K and V for one small tile: the row kernel. More
+  // rows go to the tensor-core kernel. With what the host knows, one launch is often enough.
+  const bool any_long = static_cast<int64_t>(max_q_len) * p.group > kTileRows;
+  const bool any_short = p.group <= kTileRows && num_requests > 1;
+  if (any_long) {
+    if (any_short) p.min_rows = kTileRows + 1;
+    const int rc = attn_launch_umma(p, head_dim, attn_ctas(), s);
+    if (rc || !any_short) return rc;
+    p.min_rows = 1;
+    p.max_rows = kTileRows;
+  }
   return head_dim == 64 ? launch_rows<64>(p, s) : launch_rows<128>(p, s);
 }

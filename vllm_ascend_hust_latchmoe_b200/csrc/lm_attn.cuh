@@ -27,8 +27,8 @@ struct AttnParams {
   const int32_t* tables;
   const int32_t* seq_lens;
   const int32_t* cu_q;
-  int32_t* counters;   // [kAttnMaxCtas], zero between launches
-  float* partial_o;    // [2 * ctas][rows][D]
+  int32_t* counters;   // [2 * kAttnMaxCtas], zero between launches
+  float* partial_o;    // [2 * ctas][rows * D]
   float* partial_ml;   // [2 * ctas][rows][2]: running maximum (log2 domain) and sum
   int32_t* err;
   int64_t q_token_stride, q_head_stride, out_token_stride, out_head_stride;
@@ -82,6 +82,13 @@ __device__ __forceinline__ int attn_blocks(int lo, int hi) {
   return hi > lo ? (hi + BLOCK - 1) / BLOCK - lo / BLOCK : 1;
 }
 
+// Row tiles per kv head that this launch makes of a request.
+template <int TILE_ROWS>
+__device__ __forceinline__ int attn_tiles(const AttnParams& p, const AttnRequest& r) {
+  const int rows = r.qlen * p.group;
+  return rows >= p.min_rows && rows <= p.max_rows ? (rows + TILE_ROWS - 1) / TILE_ROWS : 0;
+}
+
 // Exclusive prefix of the requests' costs in s_prefix[0 .. B]. Called by all NT threads.
 template <int TILE_ROWS, int BLOCK, int NT>
 __device__ __forceinline__ void attn_prefix(const AttnParams& p, int32_t* s_prefix, int32_t* s_warp) {
@@ -91,15 +98,12 @@ __device__ __forceinline__ void attn_prefix(const AttnParams& p, int32_t* s_pref
   int sum = 0;
   for (int b = b0; b < b1; ++b) {
     const AttnRequest r = attn_request(p, b, blockIdx.x == 0);
-    const int rows = r.qlen * p.group;
+    const int tiles = attn_tiles<TILE_ROWS>(p, r);
     int cost = 0;
-    if (rows >= p.min_rows && rows <= p.max_rows) {
-      const int tiles = (rows + TILE_ROWS - 1) / TILE_ROWS;
-      for (int t = 0; t < tiles; ++t) {
-        int lo, hi;
-        attn_tile_keys<TILE_ROWS>(p, r, t, lo, hi);
-        cost += attn_blocks<BLOCK>(lo, hi);
-      }
+    for (int t = 0; t < tiles; ++t) {
+      int lo, hi;
+      attn_tile_keys<TILE_ROWS>(p, r, t, lo, hi);
+      cost += attn_blocks<BLOCK>(lo, hi);
     }
     s_prefix[b + 1] = cost * p.kv_heads;
     sum += cost * p.kv_heads;
@@ -123,49 +127,78 @@ __device__ __forceinline__ void attn_prefix(const AttnParams& p, int32_t* s_pref
   __syncthreads();
 }
 
-// A CTA's piece of an item: kv blocks [blk0, blk1) of those that hold keys [lo, hi).
-struct AttnSegment {
+// Where a CTA stands in the launch's units: item (b, head, tile), `off` of its units already passed.
+struct AttnCursor {
   AttnRequest req;
-  int b, head, tile;
-  int lo, hi;      // keys of the whole tile
-  int blk0, blk1;  // absolute kv block numbers of this segment
-  int start, end;  // the item's units [start, end) in the launch's order
-  bool whole;
+  int b, head, tile, tiles, off;
 };
 
-// The segment at unit w of a CTA whose units end at w_end; every thread computes it alike.
+// The cursor at unit w (w < s_prefix[B]); every thread computes it alike.
 template <int TILE_ROWS, int BLOCK>
-__device__ __forceinline__ AttnSegment attn_segment(const AttnParams& p, const int32_t* s_prefix,
-                                                    int w, int w_end) {
+__device__ __forceinline__ AttnCursor attn_seek(const AttnParams& p, const int32_t* s_prefix, int w) {
   int lo_b = 0, hi_b = p.num_requests;
   while (hi_b - lo_b > 1) {  // the last request that starts at or before w; costless ones end there
     const int mid = (lo_b + hi_b) >> 1;
     if (s_prefix[mid] <= w) lo_b = mid; else hi_b = mid;
   }
-  AttnSegment s;
-  s.b = lo_b;
-  s.req = attn_request(p, lo_b, false);
-  int off = w - s_prefix[lo_b];
+  AttnCursor c;
+  c.b = lo_b;
+  c.req = attn_request(p, lo_b, false);
+  c.tiles = attn_tiles<TILE_ROWS>(p, c.req);
+  c.off = w - s_prefix[lo_b];
   const int per_head = (s_prefix[lo_b + 1] - s_prefix[lo_b]) / p.kv_heads;
-  s.head = off / per_head;
-  off -= s.head * per_head;
-  s.tile = 0;
-  int n;
-  for (;;) {
-    attn_tile_keys<TILE_ROWS>(p, s.req, s.tile, s.lo, s.hi);
-    n = attn_blocks<BLOCK>(s.lo, s.hi);
-    if (off < n) break;
-    off -= n;
-    ++s.tile;
+  c.head = c.off / per_head;
+  c.off -= c.head * per_head;
+  for (c.tile = 0;; ++c.tile) {
+    int lo, hi;
+    attn_tile_keys<TILE_ROWS>(p, c.req, c.tile, lo, hi);
+    const int n = attn_blocks<BLOCK>(lo, hi);
+    if (c.off < n) break;
+    c.off -= n;
   }
-  s.start = w - off;
+  return c;
+}
+
+// To the next item; only called when there is one.
+template <int TILE_ROWS>
+__device__ __forceinline__ void attn_advance(const AttnParams& p, AttnCursor& c) {
+  c.off = 0;
+  if (++c.tile < c.tiles) return;
+  c.tile = 0;
+  if (++c.head < p.kv_heads) return;
+  c.head = 0;
+  do {
+    ++c.b;
+    c.req = attn_request(p, c.b, false);
+    c.tiles = attn_tiles<TILE_ROWS>(p, c.req);
+  } while (c.tiles == 0 && c.b + 1 < p.num_requests);
+}
+
+// A CTA's piece of the cursor's item: kv blocks [blk0, blk1) of those that hold keys [lo, hi).
+struct AttnSegment {
+  int lo, hi;      // keys of the whole tile
+  int blk0, blk1;  // absolute kv block numbers of this segment
+  int start, end;  // the item's units [start, end) in the launch's order
+  int units;       // of this segment
+  bool whole;
+};
+
+template <int TILE_ROWS, int BLOCK>
+__device__ __forceinline__ AttnSegment attn_segment(const AttnParams& p, const AttnCursor& c, int w,
+                                                    int w_end) {
+  AttnSegment s;
+  attn_tile_keys<TILE_ROWS>(p, c.req, c.tile, s.lo, s.hi);
+  const int n = attn_blocks<BLOCK>(s.lo, s.hi);
+  s.start = w - c.off;
   s.end = s.start + n;
-  const int u1 = min(n, off + w_end - w);
-  s.whole = off == 0 && u1 == n;
-  const int first = s.lo / BLOCK;
-  s.blk0 = first + off;
-  s.blk1 = s.hi > s.lo ? first + u1 : s.blk0;
+  s.units = min(n - c.off, w_end - w);
+  s.whole = c.off == 0 && s.units == n;
+  s.blk0 = s.lo / BLOCK + c.off;
+  s.blk1 = s.hi > s.lo ? s.blk0 + s.units : s.blk0;
   return s;
 }
+
+// The launches of lm_paged_attention (lm_attn_umma.cu).
+int attn_launch_umma(const AttnParams& p, int head_dim, int ctas, cudaStream_t s);
 
 }  // namespace lm

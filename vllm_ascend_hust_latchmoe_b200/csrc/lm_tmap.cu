@@ -49,6 +49,8 @@ MapCache& map_cache() {
 
 }  // namespace
 
+PFN_cuTensorMapEncodeTiled_v12000 tensor_map_encode_fn() { return encode_fn(); }
+
 int make_map(CUtensorMap* out, const void* ptr, int rank, uint64_t d0, uint64_t d1,
              int box_rows, int box_depth) {
   const MapKey key{ptr, {d0, d1}, rank, box_rows, box_depth};

@@ -17,4 +17,7 @@ namespace lm {
 int make_map(CUtensorMap* out, const void* ptr, int rank, uint64_t d0, uint64_t d1,
              int box_rows = 128, int box_depth = 1);
 
+// The driver's cuTensorMapEncodeTiled, for maps of other shapes (null if there is none).
+PFN_cuTensorMapEncodeTiled_v12000 tensor_map_encode_fn();
+
 }  // namespace lm
