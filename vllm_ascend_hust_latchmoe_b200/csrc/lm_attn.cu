@@ -5,24 +5,27 @@
 // (fp32, in the log2 domain).
 //
 // This kernel takes 16-row tiles: single tokens and small chunks, where reading K and V is the
-// cost. The 8 warps of a CTA read 16 keys each of a 128-key block and keep their own running
-// results, so the key loop has no CTA barrier: every warp has its own 3-deep cp.async ring. Warps
-// are merged in shared memory at the end of a segment, segments of an item that several CTAs
-// share through the workspace, by the CTA that arrives last, in the order of the keys.
-#include <mutex>
+// cost. Two loader warps stream 128-key blocks of K and of V by TMA (a box per page, or per 128 keys
+// of a larger one) into a ring of three 64 KB stages and run ahead into the CTA's next segments, so
+// that the stream does not stop where a segment ends. Of a block each of 8 consumer warps takes 16
+// keys and keeps its own running results; they are merged in shared memory (over the stage that
+// they read last) at the end of a segment. Segments of an item that several CTAs share are merged
+// through the workspace, by the CTA that arrives last, in the order of the keys.
 #include <string>
 
 #include "lm_attn.cuh"
+#include "lm_tmap.cuh"
 
 namespace lm {
 namespace {
 
-constexpr int kWarps = 8;
-constexpr int kThreads = kWarps * 32;
+constexpr int kWarps = 8;       // consumers
+constexpr int kConsumerThreads = kWarps * 32;
+constexpr int kThreads = (kWarps + 3) * 32;  // and a loader each for K, V and Q
 constexpr int kTileRows = 16;
-constexpr int kSlice = 16;               // keys per warp and stage
-constexpr int kBlock = kWarps * kSlice;  // keys per unit
-constexpr int kStages = 3;
+constexpr int kSlice = 16;  // keys per warp and block
+constexpr int kBlock = kAttnBlock;
+static_assert(kBlock == kWarps * kSlice, "a slice of every block per warp");
 
 __device__ __forceinline__ void ldmatrix_x4(uint32_t (&r)[4], uint32_t addr) {
   asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];"
@@ -47,114 +50,144 @@ __device__ __forceinline__ void mma_bf16(float (&d)[4], const uint32_t (&a)[4], 
 
 template <int D>
 struct RowsSmem {
-  static constexpr int kRowBytes = D * 2;
-  static constexpr int kTile = kSlice * kRowBytes;       // K or V of one warp stage
-  static constexpr int kStage = 2 * kTile;
-  static constexpr int kRing = kWarps * kStages * kStage;
-  // merge area over the ring: O [kWarps][16][D] fp32, then m and l [kWarps][16][2]
-  static constexpr int kMerge = kWarps * kTileRows * D * 4 + kWarps * kTileRows * 2 * 4;
-  static constexpr int kBytes = kRing > kMerge ? kRing : kMerge;
+  static constexpr int kStages = D == 128 ? 3 : 6;
+  static constexpr int kHalf = kBlock * 128;         // 128 keys of 64 values
+  static constexpr int kTile = kHalf * (D / 64);     // K or V of a block
+  static constexpr int kStage = 2 * kTile;           // also 8 warps' 16 rows of D fp32
+  static constexpr int kRing = kStages * kStage;
+  static constexpr int kQ = kTileRows * D * 2;
+  static constexpr int kBytes = kRing + 2 * kQ + 1024;
 };
 
-// 16-byte chunk c of row r, XOR-swizzled so that 8 rows of one chunk column hit 8 bank groups.
+struct RowsCtrl {
+  uint64_t full[8], empty[8];
+  uint64_t q_full[2], q_empty[2];
+  float ml[kWarps][kTileRows][2];
+  int abort_flag;
+  int last;
+};
+
+// 16-byte chunk c of key row r of a K or V tile, as TMA's 128-byte swizzle lays it.
 template <int D>
-__device__ __forceinline__ uint32_t swz(int r, int c) {
+__device__ __forceinline__ uint32_t kv_at(int r, int c) {
+  return static_cast<uint32_t>((c >> 3) * RowsSmem<D>::kHalf + r * 128 + (((c ^ r) & 7) << 4));
+}
+
+// The same of a row of Q, [16][D].
+template <int D>
+__device__ __forceinline__ uint32_t q_at(int r, int c) {
   return static_cast<uint32_t>(r * (D * 2) + ((c ^ (r & 7)) << 4));
 }
 
+__device__ __forceinline__ void consumer_sync() {
+  asm volatile("bar.sync 1, %0;" ::"n"(kConsumerThreads) : "memory");
+}
+
 template <int D>
-__global__ void __launch_bounds__(kThreads, 1) paged_attn_rows_kernel(const AttnParams p) {
+__global__ void __launch_bounds__(kThreads, 1)
+    paged_attn_rows_kernel(const __grid_constant__ AttnLaunch up) {
   using S = RowsSmem<D>;
+  const AttnParams& p = up.a;
+  constexpr int kChunks = D / 8;  // 16-byte chunks per row
+  extern __shared__ unsigned char smem_raw[];
+  __shared__ int32_t s_warp[kThreads / 32];
+  __shared__ RowsCtrl c;
+  unsigned char* smem = reinterpret_cast<unsigned char*>(
+      (reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~static_cast<uintptr_t>(1023));
+  unsigned char* s_q = smem + S::kRing;
+  int32_t* s_prefix = reinterpret_cast<int32_t*>(s_q + 2 * S::kQ);
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < S::kStages; ++i) {
+      mbar_init(&c.full[i], 2);
+      mbar_init(&c.empty[i], kWarps);
+    }
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(&c.q_full[i], 32);
+      mbar_init(&c.q_empty[i], kWarps);
+    }
+    c.abort_flag = 0;
+    fence_mbarrier_init();
+  }
+  if (warp == kWarps && lane == 0) {
+    tma_prefetch_desc(&up.maps.k);
+    tma_prefetch_desc(&up.maps.v);
+  }
   pdl_wait();
   pdl_trigger();
-  extern __shared__ __align__(128) unsigned char smem[];
-  __shared__ int32_t s_warp[kWarps];
-  __shared__ int s_last;
-  int32_t* s_prefix = reinterpret_cast<int32_t*>(smem + S::kBytes);
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int g = lane >> 2, c2 = (lane & 3) * 2;
-
-  attn_prefix<kTileRows, kBlock, kThreads>(p, s_prefix, s_warp);
+  attn_prefix<kTileRows, kBlock, kThreads>(p, s_prefix, s_warp);  // its barrier covers the inits too
   const int total = s_prefix[p.num_requests];
   const int per = (total + gridDim.x - 1) / gridDim.x;
   int w = blockIdx.x * per;
   const int w_end = min(total, w + per);
-  AttnCursor at{};
-  if (w < w_end) at = attn_seek<kTileRows, kBlock>(p, s_prefix, w);
+  if (w >= w_end) return;  // the whole CTA
+  AttnCursor at = attn_seek<kTileRows, kBlock>(p, s_prefix, w);
+  volatile int* abort_flag = &c.abort_flag;
 
-  unsigned char* ring = smem + warp * kStages * S::kStage;
-  const uint32_t ring_addr = smem_u32(ring);
+  if (warp == kWarps) {
+    attn_load_kv<D, kTileRows, S::kStages, 0>(up, at, w, w_end, smem, S::kStage, c.full, c.empty, abort_flag);
+    return;
+  }
+  if (warp == kWarps + 1) {
+    attn_load_kv<D, kTileRows, S::kStages, 1>(up, at, w, w_end, smem + S::kTile, S::kStage, c.full, c.empty,
+                                              abort_flag);
+    return;
+  }
+  if (warp > kWarps) {
+    // ------------------------------------------------------------------------ queries
+    for (int seg = 0; w < w_end; ++seg) {
+      const AttnSegment s = attn_segment<kTileRows, kBlock>(p, at, w, w_end);
+      if (s.blk1 > s.blk0) {
+        if (!warp_wait(&c.q_empty[seg & 1], ((seg >> 1) & 1) ^ 1u, p.err, abort_flag)) break;
+        const int rows = at.req.qlen * p.group;
+        unsigned char* dst = s_q + (seg & 1) * S::kQ;
+#pragma unroll
+        for (int j = 0; j < kTileRows * kChunks / 32; ++j) {
+          const int r = (j * 32 + lane) / kChunks, ch = (j * 32 + lane) % kChunks;
+          const int row = at.tile * kTileRows + r;
+          const int t = row / p.group, head = at.head * p.group + row - t * p.group;
+          const uint16_t* src = p.q + (at.req.q0 + t) * p.q_token_stride + head * p.q_head_stride + ch * 8;
+          cp_async_16(dst + q_at<D>(r, ch), row < rows ? src : p.q, row < rows ? 16u : 0u);
+        }
+        cp_async_arrive_noinc(&c.q_full[seg & 1]);
+      }
+      w += s.units;
+      if (w < w_end) attn_advance<kTileRows>(p, at);
+    }
+    cp_async_wait_all();  // nothing in flight into shared memory when the warp leaves
+    return;
+  }
 
-  while (w < w_end) {
+  // -------------------------------------------------------------------------- consumers
+  // A wait that gave up is recorded and stops the loaders; the consumers go on to the end over
+  // whatever their stages hold (every later wait returns at once), so that their barriers match.
+  const int g = lane >> 2, c2 = (lane & 3) * 2;
+  int seq = 0;
+  for (int seg = 0; w < w_end; ++seg) {
     const AttnSegment s = attn_segment<kTileRows, kBlock>(p, at, w, w_end);
     const int rows = at.req.qlen * p.group;
     const int row_base = at.tile * kTileRows;
     const int cached = at.req.seq - at.req.qlen;
     const int n_slices = s.blk1 - s.blk0;  // one slice of this warp per block
-    const int32_t* table = p.tables + at.b * p.table_stride;
-    const uint16_t* kh = p.k + at.head * p.k_head_stride;
-    const uint16_t* vh = p.v + at.head * p.v_head_stride;
-    int pages = 0, page_first = 0;  // lane i: the page of slice page_first + i
 
-    auto load = [&](int i) {  // slice i of this warp into stage i % kStages
-      if (i < n_slices) {
-        if (i % 32 == 0) {
-          const int tok = (s.blk0 + i + lane) * kBlock + warp * kSlice;
-          pages = -1;
-          if (i + lane < n_slices && tok < s.hi && tok + kSlice > s.lo) {
-            pages = table[tok / p.page_size];
-            if (pages < 0 || pages >= p.num_pages) {
-              record_error(p.err, LM_DEVERR_BAD_PAGE);
-              pages = -1;
-            }
-          }
-          page_first = i;
-        }
-        const int page = __shfl_sync(0xffffffffu, pages, i - page_first);
-        const int tok0 = (s.blk0 + i) * kBlock + warp * kSlice;
-        const int in_page = tok0 % p.page_size;
-        const uint16_t* ks = kh + page * p.k_page_stride;
-        const uint16_t* vs = vh + page * p.v_page_stride;
-        unsigned char* st = ring + (i % kStages) * S::kStage;
-        constexpr int kChunks = D / 8;             // 16-byte chunks per row
-        constexpr int kIters = kSlice * kChunks / 32;
+    uint32_t qf[D / 16][4];
+    if (n_slices > 0) {
+      mbar_wait_bounded(&c.q_full[seg & 1], (seg >> 1) & 1, p.err, abort_flag);
+      const uint32_t qa = smem_u32(s_q + (seg & 1) * S::kQ);
 #pragma unroll
-        for (int j = 0; j < kIters; ++j) {
-          const int r = (j * 32 + lane) / kChunks, c = (j * 32 + lane) % kChunks;
-          // keys outside the tile's range are zeros: what the cache holds there may be anything
-          const uint32_t n = page >= 0 && tok0 + r >= s.lo && tok0 + r < s.hi ? 16u : 0u;
-          const int64_t tk = in_page + r;
-          cp_async_16(st + swz<D>(r, c), n ? ks + tk * p.k_token_stride + c * 8 : p.k, n);
-          cp_async_16(st + S::kTile + swz<D>(r, c), n ? vs + tk * p.v_token_stride + c * 8 : p.v, n);
-        }
-      }
-      asm volatile("cp.async.commit_group;" ::: "memory");
-    };
+      for (int k = 0; k < D / 16; ++k)  // rows 0-7, 8-15, then the same 8 columns on
+        ldmatrix_x4(qf[k], qa + q_at<D>(lane & 15, 2 * k + (lane >> 4)));
+    }
+    __syncwarp();
+    // a segment without keys passes its turn, so that the parities stay with the segment number
+    if (lane == 0) mbar_arrive(&c.q_empty[seg & 1]);
+    if (n_slices == 0 && warp == 0) cp_async_arrive_noinc(&c.q_full[seg & 1]);
 
-#pragma unroll
-    for (int i = 0; i < kStages - 1; ++i) load(i);
-
-    // Q fragments: rows g and g + 8 of the tile
+    // keys (j > low, j <= high) that rows g and g + 8 of the tile see
     const int r0 = row_base + g, r1 = r0 + 8;
     const int t0 = r0 / p.group, t1 = r1 / p.group;
-    uint32_t qf[D / 16][4];
-    {
-      const bool ok0 = r0 < rows, ok1 = r1 < rows;
-      const uint16_t* q0 = p.q + (at.req.q0 + t0) * p.q_token_stride +
-                           (at.head * p.group + r0 % p.group) * p.q_head_stride;
-      const uint16_t* q1 = p.q + (at.req.q0 + t1) * p.q_token_stride +
-                           (at.head * p.group + r1 % p.group) * p.q_head_stride;
-#pragma unroll
-      for (int k = 0; k < D / 16; ++k) {
-        qf[k][0] = ok0 ? *reinterpret_cast<const uint32_t*>(q0 + k * 16 + c2) : 0u;
-        qf[k][1] = ok1 ? *reinterpret_cast<const uint32_t*>(q1 + k * 16 + c2) : 0u;
-        qf[k][2] = ok0 ? *reinterpret_cast<const uint32_t*>(q0 + k * 16 + c2 + 8) : 0u;
-        qf[k][3] = ok1 ? *reinterpret_cast<const uint32_t*>(q1 + k * 16 + c2 + 8) : 0u;
-      }
-    }
-    // keys (j > low, j <= high) that the two rows see
-    const int high0 = r0 < rows ? min(cached + t0, s.hi - 1) : -1;
-    const int high1 = r1 < rows ? min(cached + t1, s.hi - 1) : -1;
+    const int high0 = r0 < rows ? cached + t0 : -1;
+    const int high1 = r1 < rows ? cached + t1 : -1;
     const int low0 = p.window > 0 ? cached + t0 - p.window : -1;
     const int low1 = p.window > 0 ? cached + t1 - p.window : -1;
 
@@ -163,22 +196,36 @@ __global__ void __launch_bounds__(kThreads, 1) paged_attn_rows_kernel(const Attn
     for (int n = 0; n < D / 8; ++n) o[n][0] = o[n][1] = o[n][2] = o[n][3] = 0.f;
     float m0 = -INFINITY, m1 = -INFINITY, l0 = 0.f, l1 = 0.f;
 
-    for (int i = 0; i < n_slices; ++i) {
-      asm volatile("cp.async.wait_group %0;" ::"n"(kStages - 2) : "memory");
-      __syncwarp();
-      load(i + kStages - 1);  // its stage was read in the last iteration, before the syncwarp
-      const uint32_t st = ring_addr + (i % kStages) * S::kStage;
+    for (int i = 0; i < n_slices; ++i, ++seq) {
+      const int stage = seq % S::kStages;
+      mbar_wait_bounded(&c.full[stage], static_cast<uint32_t>(seq / S::kStages) & 1u, p.err, abort_flag);
+      unsigned char* tile = smem + stage * S::kStage;
+      const uint32_t kt = smem_u32(tile), vt = kt + S::kTile;
+      const int tok0 = (s.blk0 + i) * kBlock + warp * kSlice;
+      if (tok0 < s.lo || tok0 + kSlice > s.hi) {
+        // V rows outside the tile's range: what the cache holds there may be anything, and a weight
+        // of zero does not undo an infinity
+        __syncwarp();
+        for (int x = lane; x < kSlice * kChunks; x += 32) {
+          const int r = x / kChunks;
+          if (tok0 + r < s.lo || tok0 + r >= s.hi)
+            *reinterpret_cast<uint4*>(tile + S::kTile + kv_at<D>(warp * kSlice + r, x % kChunks)) =
+                make_uint4(0, 0, 0, 0);
+        }
+        fence_async_shared();  // ahead of the copy that fills the stage again
+        __syncwarp();
+      }
       float sc[2][4];
 #pragma unroll
       for (int n = 0; n < 2; ++n) sc[n][0] = sc[n][1] = sc[n][2] = sc[n][3] = 0.f;
 #pragma unroll
       for (int k = 0; k < D / 16; ++k) {
         uint32_t b[4];  // keys 0-7: k halves 0, 1; keys 8-15: k halves 0, 1
-        ldmatrix_x4(b, st + swz<D>((lane & 7) + ((lane & 16) >> 1), 2 * k + ((lane >> 3) & 1)));
+        ldmatrix_x4(b, kt + kv_at<D>(warp * kSlice + (lane & 7) + ((lane & 16) >> 1), 2 * k + ((lane >> 3) & 1)));
         mma_bf16(sc[0], qf[k], b[0], b[1]);
         mma_bf16(sc[1], qf[k], b[2], b[3]);
       }
-      const int j0 = (s.blk0 + i) * kBlock + warp * kSlice + c2;
+      const int j0 = tok0 + c2;
       float mx0 = -INFINITY, mx1 = -INFINITY;
 #pragma unroll
       for (int n = 0; n < 2; ++n)
@@ -225,102 +272,132 @@ __global__ void __launch_bounds__(kThreads, 1) paged_attn_rows_kernel(const Attn
 #pragma unroll
       for (int n = 0; n < D / 16; ++n) {
         uint32_t b[4];  // d columns 16 n .. +7: keys 0-7, 8-15; columns +8: the same
-        ldmatrix_x4_trans(b, st + S::kTile + swz<D>(lane & 15, 2 * n + (lane >> 4)));
+        ldmatrix_x4_trans(b, vt + kv_at<D>(warp * kSlice + (lane & 15), 2 * n + (lane >> 4)));
         mma_bf16(o[2 * n], pa, b[0], b[1]);
         mma_bf16(o[2 * n + 1], pa, b[2], b[3]);
       }
       __syncwarp();
+      // the last stage of the segment is kept: the results go there
+      if (lane == 0 && i + 1 < n_slices) mbar_arrive(&c.empty[stage]);
     }
-    asm volatile("cp.async.wait_all;" ::: "memory");
 #pragma unroll
     for (int x = 1; x < 4; x <<= 1) {
       l0 += __shfl_xor_sync(0xffffffffu, l0, x);
       l1 += __shfl_xor_sync(0xffffffffu, l1, x);
     }
-    __syncthreads();  // every warp is done with its ring: the merge area lies over it
-
-    float* s_o = reinterpret_cast<float*>(smem);
-    float* s_ml = s_o + kWarps * kTileRows * D;
+    const int last_stage = (seq + S::kStages - 1) % S::kStages;
+    float* results = reinterpret_cast<float*>(smem + last_stage * S::kStage);  // [kWarps][16][D]
+    consumer_sync();  // every warp is done with the segment's last block
+    if (n_slices > 0) {
+      float* dst = results + warp * kTileRows * D;
 #pragma unroll
-    for (int n = 0; n < D / 8; ++n) {
-      float* d0 = s_o + (warp * kTileRows + g) * D + n * 8 + c2;
-      *reinterpret_cast<float2*>(d0) = make_float2(o[n][0], o[n][1]);
-      *reinterpret_cast<float2*>(d0 + 8 * D) = make_float2(o[n][2], o[n][3]);
+      for (int n = 0; n < D / 8; ++n) {
+        // columns in blocks of 8, swapped by row: 8 rows of one block would share their banks
+        *reinterpret_cast<float2*>(dst + g * D + (n ^ g) * 8 + c2) = make_float2(o[n][0], o[n][1]);
+        *reinterpret_cast<float2*>(dst + (g + 8) * D + (n ^ g) * 8 + c2) = make_float2(o[n][2], o[n][3]);
+      }
+      fence_async_shared();
     }
     if ((lane & 3) == 0) {
-      s_ml[(warp * kTileRows + g) * 2] = m0;
-      s_ml[(warp * kTileRows + g) * 2 + 1] = l0;
-      s_ml[(warp * kTileRows + g + 8) * 2] = m1;
-      s_ml[(warp * kTileRows + g + 8) * 2 + 1] = l1;
+      c.ml[warp][g][0] = m0;
+      c.ml[warp][g][1] = l0;
+      c.ml[warp][g + 8][0] = m1;
+      c.ml[warp][g + 8][1] = l1;
     }
-    __syncthreads();
+    consumer_sync();
 
     // 16 threads per row, D / 16 columns each
-    const int r = threadIdx.x >> 4, col = (threadIdx.x & 15) * (D / 16);
-    float m = -INFINITY, l = 0.f, acc[D / 16];
+    constexpr int kCols = D / 16;
+    const int r = threadIdx.x >> 4, col = (threadIdx.x & 15) * kCols;
+    const bool live = row_base + r < rows;
+    float m = -INFINITY, l = 0.f, acc[kCols];
 #pragma unroll
-    for (int k = 0; k < kWarps; ++k) m = fmaxf(m, s_ml[(k * kTileRows + r) * 2]);
+    for (int e = 0; e < kCols; ++e) acc[e] = 0.f;
+    if (n_slices > 0) {
 #pragma unroll
-    for (int e = 0; e < D / 16; ++e) acc[e] = 0.f;
+      for (int k = 0; k < kWarps; ++k) m = fmaxf(m, c.ml[k][r][0]);
 #pragma unroll
-    for (int k = 0; k < kWarps; ++k) {
-      const float mk = s_ml[(k * kTileRows + r) * 2];
-      const float f = mk == -INFINITY ? 0.f : exp2f(mk - m);
-      l += f * s_ml[(k * kTileRows + r) * 2 + 1];
-      const float* src = s_o + (k * kTileRows + r) * D + col;
+      for (int k = 0; k < kWarps; ++k) {
+        const float mk = c.ml[k][r][0];
+        const float f = mk == -INFINITY ? 0.f : exp2f(mk - m);
+        l += f * c.ml[k][r][1];
+        const float* src = results + (k * kTileRows + r) * D + (((col >> 3) ^ (r & 7)) * 8 + (col & 7));
 #pragma unroll
-      for (int e = 0; e < D / 16; ++e) acc[e] += f * src[e];
+        for (int e = 0; e < kCols; e += 4) {
+          const float4 v = *reinterpret_cast<const float4*>(src + e);
+          acc[e] += f * v.x;
+          acc[e + 1] += f * v.y;
+          acc[e + 2] += f * v.z;
+          acc[e + 3] += f * v.w;
+        }
+      }
     }
+    consumer_sync();  // the stages and ml have been read
+    if (n_slices > 0 && lane == 0) mbar_arrive(&c.empty[last_stage]);
 
     bool final = s.whole;
     if (!s.whole) {
       const int cs = s.start / per, ce = (s.end - 1) / per;
       const int me = blockIdx.x;
       const int64_t slot = 2 * static_cast<int64_t>(me) + (me == cs ? 1 : 0);
-      float* po = p.partial_o + (slot * kTileRows + r) * D + col;
+      if (live) {
+        float* po = p.partial_o + (slot * kTileRows + r) * D + col;
 #pragma unroll
-      for (int e = 0; e < D / 16; ++e) po[e] = acc[e];
-      if ((threadIdx.x & 15) == 0) {
-        p.partial_ml[(slot * kTileRows + r) * 2] = m;
-        p.partial_ml[(slot * kTileRows + r) * 2 + 1] = l;
+        for (int e = 0; e < kCols; e += 4)
+          *reinterpret_cast<float4*>(po + e) = make_float4(acc[e], acc[e + 1], acc[e + 2], acc[e + 3]);
+        if ((threadIdx.x & 15) == 0)
+          *reinterpret_cast<float2*>(p.partial_ml + (slot * kTileRows + r) * 2) = make_float2(m, l);
       }
       __threadfence();
-      __syncthreads();
+      consumer_sync();
       if (threadIdx.x == 0) {
-        s_last = atomicAdd(p.counters + cs, 1) == ce - cs;
-        if (s_last) p.counters[cs] = 0;  // every other CTA of the item has arrived
+        c.last = atomicAdd(p.counters + cs, 1) == ce - cs;
+        if (c.last) p.counters[cs] = 0;  // every other CTA of the item has arrived
       }
-      __syncthreads();
-      if (s_last) {
+      consumer_sync();
+      final = c.last != 0;
+      if (final && live) {
         __threadfence();
-        final = true;
+        // the common maximum first (a row's 16 threads share the partials), so that the sums'
+        // loads do not wait for one another
+        auto slot_of = [&](int k) { return (2 * static_cast<int64_t>(k) + (k == cs ? 1 : 0)) * kTileRows + r; };
+        auto ml_of = [&](int k) {
+          return __ldcg(reinterpret_cast<const float2*>(p.partial_ml + slot_of(k) * 2));
+        };
+        const unsigned group = 0xffffu << (lane & 16);
         m = -INFINITY;
+        for (int k = cs + (threadIdx.x & 15); k <= ce; k += 16) m = fmaxf(m, ml_of(k).x);
+#pragma unroll
+        for (int x = 1; x < 16; x <<= 1) m = fmaxf(m, __shfl_xor_sync(group, m, x));
         l = 0.f;
 #pragma unroll
-        for (int e = 0; e < D / 16; ++e) acc[e] = 0.f;
-        for (int c = cs; c <= ce; ++c) {
-          const int64_t sl = 2 * static_cast<int64_t>(c) + (c == cs ? 1 : 0);
-          const float mk = p.partial_ml[(sl * kTileRows + r) * 2];
-          const float lk = p.partial_ml[(sl * kTileRows + r) * 2 + 1];
-          const float mn = fmaxf(m, mk);
-          const float fa = m == -INFINITY ? 0.f : exp2f(m - mn);
-          const float fb = mk == -INFINITY ? 0.f : exp2f(mk - mn);
-          const float* src = p.partial_o + (sl * kTileRows + r) * D + col;
-          l = l * fa + lk * fb;
+        for (int e = 0; e < kCols; ++e) acc[e] = 0.f;
+#pragma unroll 8
+        for (int k = cs; k <= ce; ++k) {
+          const float2 ml = ml_of(k);
+          const float f = ml.x == -INFINITY ? 0.f : exp2f(ml.x - m);
+          const float* src = p.partial_o + slot_of(k) * D + col;
+          l += f * ml.y;
 #pragma unroll
-          for (int e = 0; e < D / 16; ++e) acc[e] = acc[e] * fa + src[e] * fb;
-          m = mn;
+          for (int e = 0; e < kCols; e += 4) {
+            const float4 v = __ldcg(reinterpret_cast<const float4*>(src + e));
+            acc[e] += f * v.x;
+            acc[e + 1] += f * v.y;
+            acc[e + 2] += f * v.z;
+            acc[e + 3] += f * v.w;
+          }
         }
       }
     }
-    if (final && row_base + r < rows) {
+    if (final && live) {
       const int tok = at.req.q0 + (row_base + r) / p.group;
       const int head = at.head * p.group + (row_base + r) % p.group;
       const float inv = l != 0.f ? 1.f / l : 0.f;
       uint16_t* dst = p.out + tok * p.out_token_stride + head * p.out_head_stride + col;
-      uint32_t packed[D / 32];
+      uint32_t packed[kCols / 2];
 #pragma unroll
-      for (int e = 0; e < D / 32; ++e) packed[e] = pack_bf16x2(acc[2 * e] * inv, acc[2 * e + 1] * inv);
+      for (int e = 0; e < kCols / 2; ++e)
+        packed[e] = pack_bf16x2(acc[2 * e] * inv, acc[2 * e + 1] * inv);
       if constexpr (D == 128)
         *reinterpret_cast<uint4*>(dst) = make_uint4(packed[0], packed[1], packed[2], packed[3]);
       else
@@ -331,7 +408,6 @@ __global__ void __launch_bounds__(kThreads, 1) paged_attn_rows_kernel(const Attn
     }
     w += s.units;
     if (w < w_end) attn_advance<kTileRows>(p, at);
-    __syncthreads();  // the merge area is free for the next segment's loads
   }
 }
 
@@ -357,9 +433,40 @@ struct Workspace {
   static int64_t bytes() { return kCounterBytes + ml_bytes() + o_bytes(); }
 };
 
+// The cache as (values, then tokens and heads by growing stride, pages); boxes of box_rows tokens of
+// one head x 64 values.
+int cache_map(CUtensorMap* out, const void* base, const AttnParams& a, int head_dim, int64_t page_stride,
+              int64_t token_stride, int64_t head_stride, int box_rows, bool heads_first) {
+  auto fn = tensor_map_encode_fn();
+  if (fn == nullptr) return fail(LM_ERR_CUDA, "cuTensorMapEncodeTiled is unavailable");
+  const int h = heads_first ? 1 : 2, t = 3 - h;
+  cuuint64_t dims[4], strides[3];
+  cuuint32_t box[4] = {64, 1, 1, 1};
+  dims[0] = static_cast<cuuint64_t>(head_dim);
+  dims[h] = static_cast<cuuint64_t>(a.kv_heads);
+  dims[t] = static_cast<cuuint64_t>(a.page_size);
+  dims[3] = static_cast<cuuint64_t>(a.num_pages);
+  strides[h - 1] = static_cast<cuuint64_t>(head_stride) * 2;
+  strides[t - 1] = static_cast<cuuint64_t>(token_stride) * 2;
+  strides[2] = static_cast<cuuint64_t>(page_stride) * 2;
+  box[t] = static_cast<cuuint32_t>(box_rows);
+  const cuuint32_t unit[4] = {1, 1, 1, 1};
+  const CUresult r = fn(out, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 4, const_cast<void*>(base), dims, strides,
+                        box, unit, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+                        CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (r != CUDA_SUCCESS)
+    return fail(LM_ERR_CUDA, "lm_paged_attention: cuTensorMapEncodeTiled failed with CUresult " +
+                                 std::to_string(r));
+  return LM_OK;
+}
+
 template <int D>
-int launch_rows(const AttnParams& p, cudaStream_t s) {
-  const size_t smem = RowsSmem<D>::kBytes + (static_cast<size_t>(p.num_requests) + 1) * 4;
+int launch_rows(const AttnParams& a, const AttnMaps& maps, cudaStream_t s) {
+  AttnLaunch p;
+  p.a = a;
+  p.maps = maps;
+  p.negate_q = 0;
+  const size_t smem = RowsSmem<D>::kBytes + (static_cast<size_t>(a.num_requests) + 1) * 4;
   static bool done[64] = {false};
   int dev = 0;
   cudaGetDevice(&dev);
@@ -378,6 +485,22 @@ int launch_rows(const AttnParams& p, cudaStream_t s) {
 }
 
 }  // namespace
+}  // namespace lm
+
+namespace lm {
+
+int attn_make_maps(const AttnParams& a, int head_dim, AttnMaps* maps) {
+  maps->box_rows = 16;
+  while (maps->box_rows < kAttnBlock && a.page_size % (2 * maps->box_rows) == 0) maps->box_rows *= 2;
+  const bool heads_first = a.k_head_stride <= a.k_token_stride && a.v_head_stride <= a.v_token_stride;
+  maps->heads_first = heads_first;
+  const int rc = cache_map(&maps->k, a.k, a, head_dim, a.k_page_stride, a.k_token_stride, a.k_head_stride,
+                           maps->box_rows, heads_first);
+  return rc ? rc
+            : cache_map(&maps->v, a.v, a, head_dim, a.v_page_stride, a.v_token_stride, a.v_head_stride,
+                        maps->box_rows, heads_first);
+}
+
 }  // namespace lm
 
 using namespace lm;
@@ -406,6 +529,7 @@ extern "C" int lm_paged_attention(
       static_cast<int64_t>(max_pages) * page_size > 0x7fffffff - 128)
     return fail(LM_ERR_INVALID_ARGUMENT, "lm_paged_attention: bad sizes (at most 4096 requests)");
   if (num_requests == 0 || num_tokens == 0) return LM_OK;
+  if (num_pages == 0) return fail(LM_ERR_INVALID_ARGUMENT, "lm_paged_attention: an empty cache");
   if (q == nullptr || k_cache == nullptr || v_cache == nullptr || block_tables == nullptr ||
       seq_lens == nullptr || cu_q == nullptr || out == nullptr || workspace == nullptr)
     return fail(LM_ERR_INVALID_ARGUMENT, "lm_paged_attention: null pointer");
@@ -462,12 +586,15 @@ extern "C" int lm_paged_attention(
   // rows go to the tensor-core kernel. With what the host knows, one launch is often enough.
   const bool any_long = static_cast<int64_t>(max_q_len) * p.group > kTileRows;
   const bool any_short = p.group <= kTileRows && num_requests > 1;
+  AttnMaps maps;
+  int rc = attn_make_maps(p, head_dim, &maps);
+  if (rc) return rc;
   if (any_long) {
     if (any_short) p.min_rows = kTileRows + 1;
-    const int rc = attn_launch_umma(p, head_dim, attn_ctas(), s);
+    rc = attn_launch_umma(p, maps, head_dim, attn_ctas(), s);
     if (rc || !any_short) return rc;
     p.min_rows = 1;
     p.max_rows = kTileRows;
   }
-  return head_dim == 64 ? launch_rows<64>(p, s) : launch_rows<128>(p, s);
+  return head_dim == 64 ? launch_rows<64>(p, maps, s) : launch_rows<128>(p, maps, s);
 }

@@ -10,6 +10,8 @@
 // continues and one of the item that it starts and does not finish.
 #pragma once
 
+#include <cuda.h>
+
 #include "lm_common.cuh"
 
 namespace lm {
@@ -198,7 +200,108 @@ __device__ __forceinline__ AttnSegment attn_segment(const AttnParams& p, const A
   return s;
 }
 
-// The launches of lm_paged_attention (lm_attn_umma.cu).
-int attn_launch_umma(const AttnParams& p, int head_dim, int ctas, cudaStream_t s);
+// A bounded wait of a whole warp, with one answer for all of its lanes.
+__device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t parity, int32_t* err,
+                                          volatile int* abort_flag) {
+  return __all_sync(0xffffffffu, mbar_wait_bounded(bar, parity, err, abort_flag));
+}
+
+// The cache as TMA sees it: K and V by boxes of box_rows tokens (a divisor of the page size, at
+// most a block) of one head x 64 values, 128-byte swizzled.
+constexpr int kAttnBlock = 128;  // keys per block
+
+struct AttnMaps {
+  CUtensorMap k, v;
+  int box_rows;
+  int heads_first;  // dimensions (values, heads, tokens, pages), else (values, tokens, heads, pages)
+};
+
+struct AttnLaunch {
+  AttnMaps maps;
+  AttnParams a;
+  int negate_q;
+};
+
+int attn_make_maps(const AttnParams& a, int head_dim, AttnMaps* maps);
+
+__device__ __forceinline__ void tma_load_4d(void* dst, const void* desc, uint64_t* bar, int32_t x,
+                                            int32_t y, int32_t z, int32_t w) {
+  asm volatile(
+      "cp.async.bulk.tensor.4d.shared::cluster.global.tile.mbarrier::complete_tx::bytes"
+      " [%0], [%1, {%3, %4, %5, %6}], [%2];" ::"r"(smem_u32(dst)),
+      "l"(desc), "r"(smem_u32(bar)), "r"(x), "r"(y), "r"(z), "r"(w)
+      : "memory");
+}
+
+__device__ __forceinline__ void fence_async_shared() {
+  asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+}
+
+// A loader warp of either kernel: the segments' blocks of K (KV 0), of V (1), or of K and V in turn
+// (2), in order, into a ring whose stages hold one tile of 128 keys ([D / 64] halves of 128 rows x
+// 128 bytes) for this warp, `stage_bytes` apart. Page ids are read a block ahead. Keys outside the
+// segment's item come from boxes past the cache's end, which TMA fills with zeros; inside a box
+// that is partly in range, the cache's own contents arrive.
+template <int D, int TILE_ROWS, int STAGES, int KV>
+__device__ __forceinline__ void attn_load_kv(const AttnLaunch& up, AttnCursor at, int w, int w_end,
+                                             unsigned char* ring, int stage_bytes, uint64_t* full,
+                                             uint64_t* empty, volatile int* abort_flag) {
+  constexpr int kHalf = kAttnBlock * 128, kTileBytes = kHalf * (D / 64);
+  const AttnParams& p = up.a;
+  const int lane = threadIdx.x & 31;
+  const int boxes = kAttnBlock / up.maps.box_rows;  // per 64 values
+  const int n_loads = boxes * (D / 64);             // one lane each, at most 16
+  const int box = lane % boxes, half = lane / boxes;
+  int seq = 0;
+  bool ok = true;
+  while (w < w_end && ok) {
+    const AttnSegment s = attn_segment<TILE_ROWS, kAttnBlock>(p, at, w, w_end);
+    const int32_t* table = p.tables + at.b * p.table_stride;
+    auto page_of = [&](int blk) {  // the page of this lane's box, num_pages where there is none
+      const int tok = blk * kAttnBlock + box * up.maps.box_rows;
+      if (lane >= n_loads || tok >= s.hi || tok + up.maps.box_rows <= s.lo) return p.num_pages;
+      const int pg = table[tok / p.page_size];
+      if (pg < 0 || pg >= p.num_pages) {
+        record_error(p.err, LM_DEVERR_BAD_PAGE);
+        return p.num_pages;
+      }
+      return pg;
+    };
+    int page = s.blk0 < s.blk1 ? page_of(s.blk0) : 0;
+    for (int blk = s.blk0; blk < s.blk1 && ok; ++blk) {
+      const int page_next = blk + 1 < s.blk1 ? page_of(blk + 1) : 0;
+      const int y = (blk * kAttnBlock + box * up.maps.box_rows) % p.page_size;
+#pragma unroll 1
+      for (int kv = KV == 1 ? 1 : 0; kv < (KV == 0 ? 1 : 2); ++kv, ++seq) {
+        const int stage = seq % STAGES;
+        const uint32_t phase = static_cast<uint32_t>(seq / STAGES) & 1u;
+        ok = warp_wait(&empty[stage], phase ^ 1u, p.err, abort_flag);
+        if (!ok) break;
+        if (lane == 0) mbar_arrive_expect_tx(&full[stage], kTileBytes);
+        __syncwarp();
+        if (lane < n_loads)
+          tma_load_4d(ring + stage * stage_bytes + half * kHalf + box * up.maps.box_rows * 128,
+                      kv == 0 ? &up.maps.k : &up.maps.v, &full[stage], half * 64,
+                      up.maps.heads_first ? at.head : y, up.maps.heads_first ? y : at.head, page);
+        __syncwarp();
+      }
+      page = page_next;
+    }
+    w += s.units;
+    if (w < w_end) attn_advance<TILE_ROWS>(p, at);
+  }
+  // every stage used is released before the CTA may leave (no copy or commit is in flight then)
+  for (int st = 0; st < STAGES && st < seq; ++st) {
+    const int last = st + ((seq - 1 - st) / STAGES) * STAGES;
+    const uint32_t par = static_cast<uint32_t>(last / STAGES) & 1u;
+    const long long t0 = clock64();
+    while (!mbar_try_wait(&empty[st], par) && clock64() - t0 < LM_SPIN_LIMIT_CYCLES) {
+      if (*abort_flag && clock64() - t0 > 200000) break;
+    }
+  }
+}
+
+// The tensor-core launch of lm_paged_attention (lm_attn_umma.cu).
+int attn_launch_umma(const AttnParams& a, const AttnMaps& maps, int head_dim, int ctas, cudaStream_t s);
 
 }  // namespace lm

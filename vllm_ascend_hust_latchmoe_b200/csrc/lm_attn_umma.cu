@@ -12,20 +12,14 @@
 // A row's reference maximum moves (and O is rescaled) only when a block's maximum exceeds it by
 // more than 2^8: exp2 of the difference then stays within fp32 and bf16 range, and the division by
 // the sum at the end takes the reference out again.
-#include <cuda.h>
-
-#include <mutex>
-#include <string>
-
 #include "lm_attn.cuh"
-#include "lm_tmap.cuh"
 
 namespace lm {
 namespace {
 
 constexpr int kRowsPerStream = 128;
 constexpr int kTile = 2 * kRowsPerStream;
-constexpr int kBlk = 128;   // keys per block
+constexpr int kBlk = kAttnBlock;
 constexpr int kThreads = 384;
 constexpr float kRescaleAbove = 8.f;  // log2
 
@@ -44,23 +38,6 @@ struct Ctrl {
   int abort_flag;
   int last[2];
 };
-
-struct UmmaAttnParams {
-  CUtensorMap k_map, v_map;
-  AttnParams a;
-  int box_rows;    // keys per TMA box: divides the page size
-  int heads_first; // the map's dimensions are (values, heads, tokens, pages), not (.., tokens, heads, ..)
-  int negate_q;
-};
-
-__device__ __forceinline__ void tma_load_4d(void* dst, const void* desc, uint64_t* bar, int32_t x,
-                                            int32_t y, int32_t z, int32_t w) {
-  asm volatile(
-      "cp.async.bulk.tensor.4d.shared::cluster.global.tile.mbarrier::complete_tx::bytes"
-      " [%0], [%1, {%3, %4, %5, %6}], [%2];" ::"r"(smem_u32(dst)),
-      "l"(desc), "r"(smem_u32(bar)), "r"(x), "r"(y), "r"(z), "r"(w)
-      : "memory");
-}
 
 // D[tmem] (+)= A[tmem] x B[smem desc], bf16 inputs, fp32 accumulate.
 __device__ __forceinline__ void umma_bf16_ts(uint32_t tmem_d, uint32_t tmem_a, uint64_t bdesc,
@@ -111,10 +88,6 @@ __device__ __forceinline__ void tmem_st_wait() {
   asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
 }
 
-__device__ __forceinline__ void fence_async_shared() {
-  asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-}
-
 __device__ __forceinline__ float ex2(float x) {
   float y;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
@@ -154,7 +127,7 @@ __device__ __forceinline__ StreamRange stream_range(const AttnParams& p, const A
 
 template <int D>
 __global__ void __launch_bounds__(kThreads, 1)
-    paged_attn_umma_kernel(const __grid_constant__ UmmaAttnParams up) {
+    paged_attn_umma_kernel(const __grid_constant__ AttnLaunch up) {
   using C = UmmaCfg<D>;
   const AttnParams& p = up.a;
   extern __shared__ unsigned char smem_raw[];
@@ -181,8 +154,8 @@ __global__ void __launch_bounds__(kThreads, 1)
     fence_mbarrier_init();
   }
   if (warp == 9 && lane == 0) {
-    tma_prefetch_desc(&up.k_map);
-    tma_prefetch_desc(&up.v_map);
+    tma_prefetch_desc(&up.maps.k);
+    tma_prefetch_desc(&up.maps.v);
   }
   pdl_wait();
   pdl_trigger();
@@ -210,58 +183,8 @@ __global__ void __launch_bounds__(kThreads, 1)
   asm volatile("setmaxnreg.dec.sync.aligned.u32 72;");
   if (warp == 9) {
     // ---------------------------------------------------------------------- K / V loader
-    const int boxes = kBlk / up.box_rows;       // per 64 values
-    const int n_loads = boxes * (D / 64);       // of one tile, one lane each (at most 16)
-    const int box = lane % boxes, half = lane / boxes;
-    int seq = 0;
-    bool ok = true;
-    for (int w = w0; w < w_end && ok;) {
-      const AttnSegment s = attn_segment<kTile, kBlk>(p, at, w, w_end);
-      const int32_t* table = p.tables + at.b * p.table_stride;
-      auto page_of = [&](int blk) {  // the page of this lane's box, num_pages where there is none
-        const int tok = blk * kBlk + box * up.box_rows;
-        if (lane >= n_loads || tok >= s.hi || tok + up.box_rows <= s.lo) return p.num_pages;
-        const int pg = table[tok / p.page_size];
-        if (pg < 0 || pg >= p.num_pages) {
-          record_error(p.err, LM_DEVERR_BAD_PAGE);
-          return p.num_pages;
-        }
-        return pg;
-      };
-      int page = s.blk0 < s.blk1 ? page_of(s.blk0) : 0;
-      for (int blk = s.blk0; blk < s.blk1 && ok; ++blk) {
-        const int page_next = blk + 1 < s.blk1 ? page_of(blk + 1) : 0;
-        const int y = (blk * kBlk + box * up.box_rows) % p.page_size;
-#pragma unroll 1
-        for (int kv = 0; kv < 2; ++kv, ++seq) {
-          const int stage = seq % C::kStages;
-          const uint32_t phase = static_cast<uint32_t>(seq / C::kStages) & 1u;
-          if (!mbar_wait_bounded(&c.kv_empty[stage], phase ^ 1u, p.err, abort_flag)) {
-            ok = false;
-            break;
-          }
-          if (lane == 0) mbar_arrive_expect_tx(&c.kv_full[stage], C::kTileBytes);
-          __syncwarp();
-          if (lane < n_loads)
-            tma_load_4d(s_kv + stage * C::kTileBytes + half * C::kHalf + box * up.box_rows * 128,
-                        kv == 0 ? &up.k_map : &up.v_map, &c.kv_full[stage], half * 64,
-                        up.heads_first ? at.head : y, up.heads_first ? y : at.head, page);
-          __syncwarp();
-        }
-        page = page_next;
-      }
-      w += s.units;
-      if (w < w_end) attn_advance<kTile>(p, at);
-    }
-    // every stage used is released before the CTA may leave (no copy or commit is in flight then)
-    for (int st = 0; st < C::kStages && st < seq; ++st) {
-      const int last = st + ((seq - 1 - st) / C::kStages) * C::kStages;
-      const uint32_t par = static_cast<uint32_t>(last / C::kStages) & 1u;
-      const long long t0 = clock64();
-      while (!mbar_try_wait(&c.kv_empty[st], par) && clock64() - t0 < LM_SPIN_LIMIT_CYCLES) {
-        if (*abort_flag && clock64() - t0 > 200000) break;
-      }
-    }
+    attn_load_kv<D, kTile, C::kStages, 2>(up, at, w0, w_end, s_kv, C::kTileBytes, c.kv_full, c.kv_empty,
+                                          abort_flag);
   } else if (warp == 8) {
     // ---------------------------------------------------------------------- MMA issuer
     const uint32_t idesc_s = idesc_bf16_f32(kRowsPerStream, kBlk);
@@ -277,7 +200,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       for (int st = 0; st < 2 && ok; ++st) {
         const StreamRange& r = st ? r1 : r0;
         if (r.end > r.begin) {
-          ok = mbar_wait_bounded(&c.q_ready[st], q_phase[st], p.err, abort_flag);
+          ok = warp_wait(&c.q_ready[st], q_phase[st], p.err, abort_flag);
           q_phase[st] ^= 1u;
         }
       }
@@ -288,10 +211,10 @@ __global__ void __launch_bounds__(kThreads, 1)
         const int k_seq = has_v ? seq + 2 : seq, v_seq = seq + 1;
         const int k_stage = has_v ? ks : seq % C::kStages;
         if (has_k)
-          ok = mbar_wait_bounded(&c.kv_full[k_stage], static_cast<uint32_t>(k_seq / C::kStages) & 1u,
+          ok = warp_wait(&c.kv_full[k_stage], static_cast<uint32_t>(k_seq / C::kStages) & 1u,
                                  p.err, abort_flag);
         if (has_v && ok) {
-          ok = mbar_wait_bounded(&c.kv_full[vs], static_cast<uint32_t>(v_seq / C::kStages) & 1u, p.err,
+          ok = warp_wait(&c.kv_full[vs], static_cast<uint32_t>(v_seq / C::kStages) & 1u, p.err,
                                  abort_flag);
           // V rows of keys outside the tile's range, in a page that is partly inside
           const int r_lo = s.lo - blk * kBlk, r_hi = s.hi - blk * kBlk;
@@ -314,7 +237,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           const StreamRange& r = st ? r1 : r0;
           const uint32_t t_s = tmem + st * 256, t_o = t_s + 128;
           if (blk >= r.begin && blk < r.end) {
-            if (!mbar_wait_bounded(&c.p_ready[st], p_phase[st], p.err, abort_flag)) {
+            if (!warp_wait(&c.p_ready[st], p_phase[st], p.err, abort_flag)) {
               ok = false;
               break;
             }
@@ -362,8 +285,9 @@ __global__ void __launch_bounds__(kThreads, 1)
     const uint32_t t_s = tmem + st * 256 + (static_cast<uint32_t>((warp & 3) * 32) << 16);
     const uint32_t t_o = t_s + 128;
     uint32_t s_phase = 0, o_phase = 0;
-    bool ok = true;
-    for (int w = w0; w < w_end && ok;) {
+    // A wait that gave up is recorded and stops the loader and the MMA warp; the rows go on to the
+    // end over whatever TMEM holds (every later wait returns at once), so that barriers match.
+    for (int w = w0; w < w_end;) {
       const AttnSegment s = attn_segment<kTile, kBlk>(p, at, w, w_end);
       const StreamRange r = stream_range(p, at, s, st);
       if (r.active) {
@@ -399,10 +323,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             p.window > 0 ? cached + (min(f_row + kRowsPerStream, rows) - 1) / p.group - p.window : -1;
         float m = -INFINITY, l = 0.f;
         for (int blk = r.begin; blk < r.end; ++blk) {
-          if (!mbar_wait_bounded(&c.s_full[st], s_phase, p.err, abort_flag)) {
-            ok = false;
-            break;
-          }
+          mbar_wait_bounded(&c.s_full[st], s_phase, p.err, abort_flag);
           s_phase ^= 1u;
           tc_fence_after();
           uint32_t x[4][32];
@@ -463,12 +384,8 @@ __global__ void __launch_bounds__(kThreads, 1)
           tc_fence_before();
           mbar_arrive(&c.p_ready[st]);
         }
-        if (!ok) break;
         if (r.end > r.begin) {
-          if (!mbar_wait_bounded(&c.o_full[st], o_phase, p.err, abort_flag)) {
-            ok = false;
-            break;
-          }
+          mbar_wait_bounded(&c.o_full[st], o_phase, p.err, abort_flag);
           o_phase ^= 1u;
           tc_fence_after();
         }
@@ -582,35 +499,8 @@ __global__ void __launch_bounds__(kThreads, 1)
   }
 }
 
-// The cache as (values, then tokens and heads by growing stride, pages); boxes of box_rows tokens of
-// one head x 64 values.
-int cache_map(CUtensorMap* out, const void* base, const AttnParams& a, int head_dim, int64_t page_stride,
-              int64_t token_stride, int64_t head_stride, int box_rows, bool heads_first) {
-  auto fn = tensor_map_encode_fn();
-  if (fn == nullptr) return fail(LM_ERR_CUDA, "cuTensorMapEncodeTiled is unavailable");
-  const int h = heads_first ? 1 : 2, t = 3 - h;
-  cuuint64_t dims[4], strides[3];
-  cuuint32_t box[4] = {64, 1, 1, 1};
-  dims[0] = static_cast<cuuint64_t>(head_dim);
-  dims[h] = static_cast<cuuint64_t>(a.kv_heads);
-  dims[t] = static_cast<cuuint64_t>(a.page_size);
-  dims[3] = static_cast<cuuint64_t>(a.num_pages);
-  strides[h - 1] = static_cast<cuuint64_t>(head_stride) * 2;
-  strides[t - 1] = static_cast<cuuint64_t>(token_stride) * 2;
-  strides[2] = static_cast<cuuint64_t>(page_stride) * 2;
-  box[t] = static_cast<cuuint32_t>(box_rows);
-  const cuuint32_t unit[4] = {1, 1, 1, 1};
-  const CUresult r = fn(out, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 4, const_cast<void*>(base), dims, strides,
-                        box, unit, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
-                        CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
-  if (r != CUDA_SUCCESS)
-    return fail(LM_ERR_CUDA, "lm_paged_attention: cuTensorMapEncodeTiled failed with CUresult " +
-                                 std::to_string(r));
-  return LM_OK;
-}
-
 template <int D>
-int launch(const UmmaAttnParams& p, int ctas, cudaStream_t s) {
+int launch(const AttnLaunch& p, int ctas, cudaStream_t s) {
   static bool done[64] = {false};
   int dev = 0;
   cudaGetDevice(&dev);
@@ -630,23 +520,15 @@ int launch(const UmmaAttnParams& p, int ctas, cudaStream_t s) {
 
 }  // namespace
 
-int attn_launch_umma(const AttnParams& a, int head_dim, int ctas, cudaStream_t s) {
-  UmmaAttnParams p;
+int attn_launch_umma(const AttnParams& a, const AttnMaps& maps, int head_dim, int ctas, cudaStream_t s) {
+  AttnLaunch p;
   p.a = a;
+  p.maps = maps;
   // Q's sign takes a negative scale's, so that a row's largest S has its largest weight; with a
   // scale of 0 the masked scores (-inf) still have to vanish.
   p.negate_q = a.scale_log2 < 0.f;
   if (p.negate_q) p.a.scale_log2 = -a.scale_log2;
   if (a.scale_log2 == 0.f) p.a.scale_log2 = 1e-30f;
-  p.box_rows = 16;
-  while (p.box_rows < kBlk && a.page_size % (2 * p.box_rows) == 0) p.box_rows *= 2;
-  p.heads_first = a.k_head_stride <= a.k_token_stride && a.v_head_stride <= a.v_token_stride;
-  int rc = cache_map(&p.k_map, a.k, a, head_dim, a.k_page_stride, a.k_token_stride, a.k_head_stride,
-                     p.box_rows, p.heads_first);
-  if (!rc)
-    rc = cache_map(&p.v_map, a.v, a, head_dim, a.v_page_stride, a.v_token_stride, a.v_head_stride,
-                   p.box_rows, p.heads_first);
-  if (rc) return rc;
   return head_dim == 64 ? launch<64>(p, ctas, s) : launch<128>(p, ctas, s);
 }
 
