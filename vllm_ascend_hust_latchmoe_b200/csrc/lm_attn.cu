@@ -124,13 +124,10 @@ __global__ void __launch_bounds__(kThreads, 1)
   AttnCursor at = attn_seek<kTileRows, kBlock>(p, s_prefix, w);
   volatile int* abort_flag = &c.abort_flag;
 
-  if (warp == kWarps) {
-    attn_load_kv<D, kTileRows, S::kStages, 0>(up, at, w, w_end, smem, S::kStage, c.full, c.empty, abort_flag);
-    return;
-  }
-  if (warp == kWarps + 1) {
-    attn_load_kv<D, kTileRows, S::kStages, 1>(up, at, w, w_end, smem + S::kTile, S::kStage, c.full, c.empty,
-                                              abort_flag);
+  if (warp < kWarps + 2 && warp >= kWarps) {
+    const bool is_v = warp == kWarps + 1;
+    attn_load_kv<D, kTileRows, S::kStages>(up, is_v, at, w, w_end, smem + (is_v ? S::kTile : 0), S::kStage, 0, 1,
+                                           c.full, c.empty, abort_flag);
     return;
   }
   if (warp > kWarps) {

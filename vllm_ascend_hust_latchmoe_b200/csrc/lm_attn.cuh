@@ -237,22 +237,25 @@ __device__ __forceinline__ void fence_async_shared() {
   asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
 }
 
-// A loader warp of either kernel: the segments' blocks of K (KV 0), of V (1), or of K and V in turn
-// (2), in order, into a ring whose stages hold one tile of 128 keys ([D / 64] halves of 128 rows x
-// 128 bytes) for this warp, `stage_bytes` apart. Page ids are read a block ahead. Keys outside the
+// A loader warp of either kernel: the segments' blocks of K or of V, in order, as tiles of 128 keys
+// ([D / 64] halves of 128 rows x 128 bytes). Its n-th tile is number first + n * step of a ring
+// with STAGES places, `stage_bytes` apart. Page ids are read a block ahead. Keys outside the
 // segment's item come from boxes past the cache's end, which TMA fills with zeros; inside a box
-// that is partly in range, the cache's own contents arrive.
-template <int D, int TILE_ROWS, int STAGES, int KV>
-__device__ __forceinline__ void attn_load_kv(const AttnLaunch& up, AttnCursor at, int w, int w_end,
-                                             unsigned char* ring, int stage_bytes, uint64_t* full,
-                                             uint64_t* empty, volatile int* abort_flag) {
+// that is partly in range, the cache's own contents arrive. One warp for both would not do: with
+// pages of 16 keys (boxes of 2 KB) a warp issues 34 GB/s.
+template <int D, int TILE_ROWS, int STAGES>
+__device__ __forceinline__ void attn_load_kv(const AttnLaunch& up, bool is_v, AttnCursor at, int w,
+                                             int w_end, unsigned char* ring, int stage_bytes, int first,
+                                             int step, uint64_t* full, uint64_t* empty,
+                                             volatile int* abort_flag) {
   constexpr int kHalf = kAttnBlock * 128, kTileBytes = kHalf * (D / 64);
   const AttnParams& p = up.a;
   const int lane = threadIdx.x & 31;
   const int boxes = kAttnBlock / up.maps.box_rows;  // per 64 values
   const int n_loads = boxes * (D / 64);             // one lane each, at most 16
   const int box = lane % boxes, half = lane / boxes;
-  int seq = 0;
+  const CUtensorMap* map = is_v ? &up.maps.v : &up.maps.k;
+  int stage = first % STAGES, passes = 0, tiles = 0;
   bool ok = true;
   while (w < w_end && ok) {
     const AttnSegment s = attn_segment<TILE_ROWS, kAttnBlock>(p, at, w, w_end);
@@ -271,29 +274,31 @@ __device__ __forceinline__ void attn_load_kv(const AttnLaunch& up, AttnCursor at
     for (int blk = s.blk0; blk < s.blk1 && ok; ++blk) {
       const int page_next = blk + 1 < s.blk1 ? page_of(blk + 1) : 0;
       const int y = (blk * kAttnBlock + box * up.maps.box_rows) % p.page_size;
-#pragma unroll 1
-      for (int kv = KV == 1 ? 1 : 0; kv < (KV == 0 ? 1 : 2); ++kv, ++seq) {
-        const int stage = seq % STAGES;
-        const uint32_t phase = static_cast<uint32_t>(seq / STAGES) & 1u;
-        ok = warp_wait(&empty[stage], phase ^ 1u, p.err, abort_flag);
-        if (!ok) break;
-        if (lane == 0) mbar_arrive_expect_tx(&full[stage], kTileBytes);
-        __syncwarp();
-        if (lane < n_loads)
-          tma_load_4d(ring + stage * stage_bytes + half * kHalf + box * up.maps.box_rows * 128,
-                      kv == 0 ? &up.maps.k : &up.maps.v, &full[stage], half * 64,
-                      up.maps.heads_first ? at.head : y, up.maps.heads_first ? y : at.head, page);
-        __syncwarp();
+      ok = warp_wait(&empty[stage], (passes & 1u) ^ 1u, p.err, abort_flag);
+      if (!ok) break;
+      if (lane == 0) mbar_arrive_expect_tx(&full[stage], kTileBytes);
+      __syncwarp();
+      if (lane < n_loads)
+        tma_load_4d(ring + stage * stage_bytes + half * kHalf + box * up.maps.box_rows * 128, map,
+                    &full[stage], half * 64, up.maps.heads_first ? at.head : y,
+                    up.maps.heads_first ? y : at.head, page);
+      __syncwarp();
+      ++tiles;
+      stage += step;
+      if (stage >= STAGES) {
+        stage -= STAGES;
+        ++passes;
       }
       page = page_next;
     }
     w += s.units;
     if (w < w_end) attn_advance<TILE_ROWS>(p, at);
   }
-  // every stage used is released before the CTA may leave (no copy or commit is in flight then)
-  for (int st = 0; st < STAGES && st < seq; ++st) {
-    const int last = st + ((seq - 1 - st) / STAGES) * STAGES;
-    const uint32_t par = static_cast<uint32_t>(last / STAGES) & 1u;
+  // Every stage used is released before the CTA may leave (no copy or commit is in flight then); of
+  // two warps that fill the ring in turn, the one that ends last sees the last pass of each stage.
+  const int total = tiles * step;
+  for (int st = 0; st < STAGES && st < total; ++st) {
+    const uint32_t par = static_cast<uint32_t>((total - 1 - st) / STAGES) & 1u;
     const long long t0 = clock64();
     while (!mbar_try_wait(&empty[st], par) && clock64() - t0 < LM_SPIN_LIMIT_CYCLES) {
       if (*abort_flag && clock64() - t0 > 200000) break;

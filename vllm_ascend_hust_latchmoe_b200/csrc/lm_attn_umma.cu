@@ -3,11 +3,11 @@
 // A CTA works on tiles of 256 rows of one (request, kv head), as two streams of 128 rows, against
 // blocks of 128 keys. S = Q K^T and O += P V are tcgen05 MMAs (fp32 accumulators in TMEM: S and O
 // of both streams fill its 512 columns); P is written back over S's columns as bf16 and read from
-// TMEM as the A operand. One warp issues the MMAs, in the order PV(0), S(0), PV(1), S(1), so the
-// tensor pipe works on one stream while the other stream's 128 softmax threads (a row each) turn
-// S into P. One warp loads K and V by TMA, a box per cache page (or per 128 keys of a larger one),
-// into a ring of 32 KB tiles; pages that are out of range are boxes past the cache's end, which
-// TMA fills with zeros, and the MMA warp zeroes the V rows past a sequence's end inside a page.
+// TMEM as the A operand. A warp per stream issues its MMAs, P V of one block and then S of the next,
+// so the tensor pipe works on one stream while the other stream's 128 softmax threads (a row each)
+// turn S into P. Two warps load K and V by TMA, a box per cache page (or per 128 keys of a larger
+// one), in turn into a ring of 32 KB tiles; pages that are out of range are boxes past the cache's end,
+// which TMA fills with zeros, and the MMA warps zero the V rows past a sequence's end inside a page.
 //
 // A row's reference maximum moves (and O is rescaled) only when a block's maximum exceeds it by
 // more than 2^8: exp2 of the difference then stays within fp32 and bf16 range, and the division by
@@ -33,7 +33,7 @@ struct UmmaCfg {
 
 struct Ctrl {
   uint64_t kv_full[8], kv_empty[8];
-  uint64_t q_ready[2], s_full[2], p_ready[2], o_full[2];
+  uint64_t q_ready[2], s_full[2], p_half[2], p_ready[2], o_full[2], turn[2];
   uint32_t tmem_base;
   int abort_flag;
   int last[2];
@@ -49,6 +49,20 @@ __device__ __forceinline__ void umma_bf16_ts(uint32_t tmem_d, uint32_t tmem_a, u
       "r"(tmem_a), "l"(bdesc), "r"(idesc), "r"(accumulate)
       : "memory");
 }
+
+// One thread of a converged warp. (Operands that the compiler can see are the same in the whole warp
+// keep an MMA's issue short: see uniform().)
+__device__ __forceinline__ bool elect_one() {
+  uint32_t r;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "elect.sync _|p, 0xffffffff;\n\t"
+      "selp.u32 %0, 1, 0, p;\n\t}"
+      : "=r"(r));
+  return r != 0;
+}
+
+__device__ __forceinline__ uint32_t uniform(uint32_t v) { return __shfl_sync(0xffffffffu, v, 0); }
 
 // Descriptor of a tile whose rows are the K dimension (128 B of 64 N values each, 128B swizzle):
 // atoms of 8 rows follow each other at 1024 B (SBO), the next 64 N values are at `n_stride` (LBO).
@@ -94,6 +108,32 @@ __device__ __forceinline__ float ex2(float x) {
   return y;
 }
 
+// Two floats in one register pair: the FMA pipe does both in one instruction.
+__device__ __forceinline__ uint64_t pair(float lo, float hi) {
+  uint64_t r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(lo), "f"(hi));
+  return r;
+}
+__device__ __forceinline__ void unpair(uint64_t v, float& lo, float& hi) {
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(lo), "=f"(hi) : "l"(v));
+}
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  return r;
+}
+__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+
+__device__ __forceinline__ float max3(float a, float b, float c) {
+  float r;
+  asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+  return r;
+}
+
 // Barrier among the 128 threads of one stream (ids 1 and 2; 0 is __syncthreads).
 __device__ __forceinline__ void stream_sync(int stream) {
   if (stream == 0)
@@ -137,18 +177,20 @@ __global__ void __launch_bounds__(kThreads, 1)
       (reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~static_cast<uintptr_t>(1023));
   unsigned char* s_q = smem;                       // [2][kTileBytes]
   unsigned char* s_kv = smem + 2 * C::kTileBytes;  // [kStages][kTileBytes]
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int warp = uniform(threadIdx.x >> 5), lane = threadIdx.x & 31;
 
   if (threadIdx.x == 0) {
     for (int i = 0; i < C::kStages; ++i) {
       mbar_init(&c.kv_full[i], 1);
-      mbar_init(&c.kv_empty[i], 1);
+      mbar_init(&c.kv_empty[i], 2);  // both streams'
     }
     for (int i = 0; i < 2; ++i) {
       mbar_init(&c.q_ready[i], kRowsPerStream);
       mbar_init(&c.s_full[i], 1);
+      mbar_init(&c.p_half[i], kRowsPerStream);
       mbar_init(&c.p_ready[i], kRowsPerStream);
       mbar_init(&c.o_full[i], 1);
+      mbar_init(&c.turn[i], 1);
     }
     c.abort_flag = 0;
     fence_mbarrier_init();
@@ -175,104 +217,128 @@ __global__ void __launch_bounds__(kThreads, 1)
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
-  const uint32_t tmem = c.tmem_base;
+  const uint32_t tmem = uniform(c.tmem_base);
   volatile int* abort_flag = &c.abort_flag;
 
   // 256 softmax threads of 216 registers and 128 others of 72: the 384 x 168 of the launch
   if (warp >= 8) {
   asm volatile("setmaxnreg.dec.sync.aligned.u32 72;");
-  if (warp == 9) {
-    // ---------------------------------------------------------------------- K / V loader
-    attn_load_kv<D, kTile, C::kStages, 2>(up, at, w0, w_end, s_kv, C::kTileBytes, c.kv_full, c.kv_empty,
-                                          abort_flag);
-  } else if (warp == 8) {
-    // ---------------------------------------------------------------------- MMA issuer
+  if (warp == 9 || warp == 11) {
+    // ---------------------------------------------------------------------- K and V loaders
+    attn_load_kv<D, kTile, C::kStages>(up, warp == 11, at, w0, w_end, s_kv, C::kTileBytes, warp == 11 ? 1 : 0, 2,
+                                       c.kv_full, c.kv_empty, abort_flag);
+  } else if (warp == 8 || warp == 10) {
+    // ---------------------------------------------------------------------- MMA issuers, one a stream
+    const int st = warp == 8 ? 0 : 1;
     const uint32_t idesc_s = idesc_bf16_f32(kRowsPerStream, kBlk);
     const uint32_t idesc_o = idesc_bf16_f32(kRowsPerStream, D) | (1u << 16);  // B is N-major
-    const uint32_t q_addr = smem_u32(s_q), kv_addr = smem_u32(s_kv);
-    uint32_t q_phase[2] = {0, 0}, p_phase[2] = {0, 0};
-    int seq = 0;  // K tiles of block n: 2 n, V tiles: 2 n + 1
+    const uint32_t kv_addr = uniform(smem_u32(s_kv));
+    const uint64_t q_desc = sdesc_k_sw128(uniform(smem_u32(s_q)) + st * C::kTileBytes);
+    const uint32_t t_s = tmem + st * 256, t_o = t_s + 128;
+    uint32_t q_phase = 0, p_phase = 0, kv_phase = 0;
+    uint32_t turn_phase = st == 0 ? 1u : 0u;  // stream 0 begins
+    int stage = 0;  // of the next tile, in the loader's order: K, V, K, V, ...
     bool ok = true;
+    auto next_stage = [&]() {
+      if (++stage == C::kStages) {
+        stage = 0;
+        kv_phase ^= 1u;
+      }
+    };
+    auto release = [&](int tile, bool used) {  // after this stream's MMAs, if it had any
+      if (elect_one()) {
+        if (used)
+          umma_commit(&c.kv_empty[tile]);
+        else
+          mbar_arrive(&c.kv_empty[tile]);
+      }
+      __syncwarp();
+    };
+    auto issue_s = [&](int tile) {
+      const uint64_t k_desc = sdesc_k_sw128(uniform(kv_addr + tile * C::kTileBytes));
+      tc_fence_after();
+      if (elect_one()) {
+#pragma unroll
+        for (int k = 0; k < D / 16; ++k) {
+          const uint64_t off = ((k / 4) * C::kHalf + (k % 4) * 32) >> 4;
+          umma_bf16(t_s, q_desc + off, k_desc + off, idesc_s, k > 0 ? 1u : 0u);
+        }
+        umma_commit(&c.s_full[st]);
+      }
+      __syncwarp();
+    };
     for (int w = w0; w < w_end && ok;) {
       const AttnSegment s = attn_segment<kTile, kBlk>(p, at, w, w_end);
-      const StreamRange r0 = stream_range(p, at, s, 0), r1 = stream_range(p, at, s, 1);
-#pragma unroll 1
-      for (int st = 0; st < 2 && ok; ++st) {
-        const StreamRange& r = st ? r1 : r0;
-        if (r.end > r.begin) {
-          ok = warp_wait(&c.q_ready[st], q_phase[st], p.err, abort_flag);
-          q_phase[st] ^= 1u;
-        }
+      const StreamRange r = stream_range(p, at, s, st);
+      if (r.end > r.begin) {
+        ok = warp_wait(&c.q_ready[st], q_phase, p.err, abort_flag);
+        q_phase ^= 1u;
       }
-      for (int blk = s.blk0 - 1; blk < s.blk1 && ok && s.blk1 > s.blk0; ++blk) {
-        // S of block blk + 1, P V of block blk
-        const int ks = (seq + 2) % C::kStages, vs = (seq + 1) % C::kStages;
-        const bool has_k = blk + 1 < s.blk1, has_v = blk >= s.blk0;
-        const int k_seq = has_v ? seq + 2 : seq, v_seq = seq + 1;
-        const int k_stage = has_v ? ks : seq % C::kStages;
-        if (has_k)
-          ok = warp_wait(&c.kv_full[k_stage], static_cast<uint32_t>(k_seq / C::kStages) & 1u,
-                                 p.err, abort_flag);
-        if (has_v && ok) {
-          ok = warp_wait(&c.kv_full[vs], static_cast<uint32_t>(v_seq / C::kStages) & 1u, p.err,
-                                 abort_flag);
-          // V rows of keys outside the tile's range, in a page that is partly inside
-          const int r_lo = s.lo - blk * kBlk, r_hi = s.hi - blk * kBlk;
-          if (ok && (r_lo > 0 || r_hi < kBlk)) {
+      if (s.blk0 < s.blk1 && ok) {  // S of the first block
+        ok = warp_wait(&c.kv_full[stage], kv_phase, p.err, abort_flag);
+        if (!ok) break;
+        const bool mine = s.blk0 == r.begin && r.end > r.begin;
+        if (mine) issue_s(stage);
+        release(stage, mine);
+        next_stage();
+      }
+      for (int blk = s.blk0; blk < s.blk1; ++blk) {  // P V of blk, S of blk + 1
+        const bool mine = blk >= r.begin && blk < r.end;
+        const int v_tile = stage;
+        const uint32_t v_phase = kv_phase;
+        next_stage();
+        if (blk + 1 < s.blk1) {
+          ok = warp_wait(&c.kv_full[stage], kv_phase, p.err, abort_flag);  // K arrives after V
+          if (!ok) break;
+        }
+        ok = warp_wait(&c.kv_full[v_tile], v_phase, p.err, abort_flag);
+        if (!ok) break;
+        // The streams take turns, so that one's softmax runs beside the other's MMAs; left alone they
+        // fall into step, and exponentials and MMAs wait for their own kind (1027 against 930 us).
+        ok = warp_wait(&c.turn[st], turn_phase, p.err, abort_flag);
+        if (!ok) break;
+        turn_phase ^= 1u;
+        if (mine) {
+          // V rows of keys outside the tile's range, in a page that is partly inside (both streams
+          // write the same zeros)
+          const int r_lo = max(0, s.lo - blk * kBlk), r_hi = min(kBlk, s.hi - blk * kBlk);
+          if (r_lo > 0 || r_hi < kBlk) {
             const uint4 zero = make_uint4(0, 0, 0, 0);
-            for (int i = lane; i < kBlk * (D / 8); i += 32) {
-              const int row = i / (D / 8), ch = i % (D / 8);
-              if (row < r_lo || row >= r_hi)
-                *reinterpret_cast<uint4*>(s_kv + vs * C::kTileBytes + (ch / 8) * C::kHalf + row * 128 +
-                                          (ch % 8) * 16) = zero;
+            for (int i = lane; i < (kBlk - (r_hi - r_lo)) * (D / 8); i += 32) {
+              const int n = i / (D / 8), ch = i % (D / 8);
+              const int row = n < r_lo ? n : n - r_lo + r_hi;
+              *reinterpret_cast<uint4*>(s_kv + v_tile * C::kTileBytes + (ch / 8) * C::kHalf + row * 128 +
+                                        (ch % 8) * 16) = zero;
             }
             fence_async_shared();
             __syncwarp();
           }
-        }
-        if (!ok) break;
-        tc_fence_after();
-#pragma unroll 1
-        for (int st = 0; st < 2; ++st) {
-          const StreamRange& r = st ? r1 : r0;
-          const uint32_t t_s = tmem + st * 256, t_o = t_s + 128;
-          if (blk >= r.begin && blk < r.end) {
-            if (!warp_wait(&c.p_ready[st], p_phase[st], p.err, abort_flag)) {
-              ok = false;
-              break;
-            }
-            p_phase[st] ^= 1u;
+          const uint64_t v_desc = sdesc_mn_sw128(uniform(kv_addr + v_tile * C::kTileBytes), C::kHalf);
+          const uint32_t accumulate = uniform(blk > r.begin ? 1u : 0u);
+#pragma unroll
+          for (int part = 0; part < 2; ++part) {
+            ok = ok && warp_wait(part ? &c.p_ready[st] : &c.p_half[st], p_phase, p.err, abort_flag);
+            if (!ok) break;
             tc_fence_after();
-            if (lane == 0) {
-              const uint32_t v = kv_addr + vs * C::kTileBytes;
+            if (elect_one()) {
 #pragma unroll
-              for (int k = 0; k < kBlk / 16; ++k)
-                umma_bf16_ts(t_o, t_s + k * 8, sdesc_mn_sw128(v + k * 2048, C::kHalf), idesc_o,
-                             (blk > r.begin || k > 0) ? 1u : 0u);
-              if (blk == r.end - 1) umma_commit(&c.o_full[st]);
+              for (int k = part * kBlk / 32; k < (part + 1) * kBlk / 32; ++k)
+                umma_bf16_ts(t_o, t_s + k * 8, v_desc + k * (2048 >> 4), idesc_o, k > 0 ? 1u : accumulate);
+              if (part == 1 && blk == r.end - 1) umma_commit(&c.o_full[st]);
             }
             __syncwarp();
           }
-          if (blk + 1 >= r.begin && blk + 1 < r.end) {
-            if (lane == 0) {
-              const uint32_t q = q_addr + st * C::kTileBytes, k0 = kv_addr + k_stage * C::kTileBytes;
-#pragma unroll
-              for (int k = 0; k < D / 16; ++k) {
-                const uint32_t off = (k / 4) * C::kHalf + (k % 4) * 32;
-                umma_bf16(t_s, sdesc_k_sw128(q + off), sdesc_k_sw128(k0 + off), idesc_s, k > 0 ? 1u : 0u);
-              }
-              umma_commit(&c.s_full[st]);
-            }
-            __syncwarp();
-          }
+          if (!ok) break;
+          p_phase ^= 1u;
         }
-        if (!ok) break;
-        if (lane == 0) {
-          if (has_v) umma_commit(&c.kv_empty[vs]);
-          if (has_k) umma_commit(&c.kv_empty[k_stage]);
+        const bool next = blk + 1 >= r.begin && blk + 1 < r.end;
+        if (next) issue_s(stage);
+        if (elect_one()) mbar_arrive(&c.turn[1 - st]);
+        release(v_tile, mine);
+        if (blk + 1 < s.blk1) {
+          release(stage, next);
+          next_stage();
         }
-        __syncwarp();
-        if (has_v) seq += 2;
       }
       w += s.units;
       if (w < w_end) attn_advance<kTile>(p, at);
@@ -340,12 +406,15 @@ __global__ void __launch_bounds__(kThreads, 1)
                 if (j > high || j <= low) x[i][e] = 0xff800000u;
               }
           }
-          float mx = -INFINITY;
+          float top[4];  // four chains: one would be 128 dependent steps
 #pragma unroll
-          for (int i = 0; i < 4; ++i)
+          for (int i = 0; i < 4; ++i) {
+            top[i] = fmaxf(__uint_as_float(x[i][0]), __uint_as_float(x[i][1]));
 #pragma unroll
-            for (int e = 0; e < 32; ++e) mx = fmaxf(mx, __uint_as_float(x[i][e]));
-          mx *= p.scale_log2;
+            for (int e = 2; e < 32; e += 2)
+              top[i] = max3(top[i], __uint_as_float(x[i][e]), __uint_as_float(x[i][e + 1]));
+          }
+          const float mx = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])) * p.scale_log2;
           const bool move = mx > m + kRescaleAbove || (m == -INFINITY && mx > m);
           if (__any_sync(0xffffffffu, move)) {
             const float nm = move ? mx : m;
@@ -365,20 +434,29 @@ __global__ void __launch_bounds__(kThreads, 1)
             }
           }
           const float base = m == -INFINITY ? 0.f : -m;
-          float sum0 = 0.f, sum1 = 0.f;
+          const uint64_t scale2 = pair(p.scale_log2, p.scale_log2), base2 = pair(base, base);
+          uint64_t sum2 = pair(0.f, 0.f);
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
             uint32_t packed[16];
 #pragma unroll
             for (int e = 0; e < 16; ++e) {
-              const float a = ex2(fmaf(__uint_as_float(x[i][2 * e]), p.scale_log2, base));
-              const float b = ex2(fmaf(__uint_as_float(x[i][2 * e + 1]), p.scale_log2, base));
-              sum0 += a;
-              sum1 += b;
+              float a, b;
+              unpair(fma2(pair(__uint_as_float(x[i][2 * e]), __uint_as_float(x[i][2 * e + 1])), scale2, base2), a, b);
+              a = ex2(a);
+              b = ex2(b);
+              sum2 = add2(sum2, pair(a, b));
               packed[e] = pack_bf16x2(a, b);
             }
             tmem_st_32x32b_x16(t_s + i * 16, packed);
+            if (i == 1) {  // P V may begin with the first half of the keys
+              tmem_st_wait();
+              tc_fence_before();
+              mbar_arrive(&c.p_half[st]);
+            }
           }
+          float sum0, sum1;
+          unpair(sum2, sum0, sum1);
           l += sum0 + sum1;
           tmem_st_wait();
           tc_fence_before();
