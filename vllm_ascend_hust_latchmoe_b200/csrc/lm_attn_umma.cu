@@ -9,9 +9,11 @@
 // one), in turn into a ring of 32 KB tiles; pages that are out of range are boxes past the cache's end,
 // which TMA fills with zeros, and the MMA warps zero the V rows past a sequence's end inside a page.
 //
-// A row's reference maximum moves (and O is rescaled) only when a block's maximum exceeds it by
-// more than 2^8: exp2 of the difference then stays within fp32 and bf16 range, and the division by
-// the sum at the end takes the reference out again.
+// A row's reference maximum moves (and O is rescaled) only when a block's maximum exceeds it by a
+// factor of more than 2^24: weights, sums and O keep their relative precision (fp32 and bf16 have 8
+// exponent bits), 2^100 of range is left for V and the number of keys, and the division by the sum
+// at the end takes the reference out again. A move costs its stream some 700 cycles, and with a
+// bound of 2^8 sharp heads moved one of 128 rows in most blocks.
 #include "lm_attn.cuh"
 
 namespace lm {
@@ -21,7 +23,7 @@ constexpr int kRowsPerStream = 128;
 constexpr int kTile = 2 * kRowsPerStream;
 constexpr int kBlk = kAttnBlock;
 constexpr int kThreads = 384;
-constexpr float kRescaleAbove = 8.f;  // log2
+constexpr float kRescaleAbove = 24.f;  // log2
 
 template <int D>
 struct UmmaCfg {
@@ -353,33 +355,39 @@ __global__ void __launch_bounds__(kThreads, 1)
     uint32_t s_phase = 0, o_phase = 0;
     // A wait that gave up is recorded and stops the loader and the MMA warp; the rows go on to the
     // end over whatever TMEM holds (every later wait returns at once), so that barriers match.
-    for (int w = w0; w < w_end;) {
-      const AttnSegment s = attn_segment<kTile, kBlk>(p, at, w, w_end);
-      const StreamRange r = stream_range(p, at, s, st);
-      if (r.active) {
-        const int rows = at.req.qlen * p.group, cached = at.req.seq - at.req.qlen;
-        const int fr = at.tile * kTile + st * kRowsPerStream + row;  // flattened row
-        const bool live = fr < rows;
-        const int t = fr / p.group, head = at.head * p.group + fr % p.group;
-        if (r.end > r.begin) {
-          const uint16_t* src = p.q + (at.req.q0 + t) * p.q_token_stride + head * p.q_head_stride;
-          const uint32_t flip = up.negate_q ? 0x80008000u : 0u;
+    // this thread's row of a segment's Q into shared memory
+    auto load_q = [&](const AttnCursor& q_at) {
+      const int fr = q_at.tile * kTile + st * kRowsPerStream + row;
+      const int t = fr / p.group, head = q_at.head * p.group + fr - t * p.group;
+      const bool live = fr < q_at.req.qlen * p.group;
+      const uint16_t* src = p.q + (q_at.req.q0 + t) * p.q_token_stride + head * p.q_head_stride;
+      const uint32_t flip = up.negate_q ? 0x80008000u : 0u;
 #pragma unroll
-          for (int ch = 0; ch < D / 8; ++ch) {
-            uint4 v = make_uint4(0, 0, 0, 0);
-            if (live) {
-              v = *reinterpret_cast<const uint4*>(src + ch * 8);
-              v.x ^= flip;
-              v.y ^= flip;
-              v.z ^= flip;
-              v.w ^= flip;
-            }
-            *reinterpret_cast<uint4*>(s_q + st * C::kTileBytes + (ch / 8) * C::kHalf + row * 128 +
-                                      (((ch % 8) ^ (row & 7)) << 4)) = v;
-          }
-          fence_async_shared();
-          mbar_arrive(&c.q_ready[st]);
+      for (int ch = 0; ch < D / 8; ++ch) {
+        uint4 v = make_uint4(0, 0, 0, 0);
+        if (live) {
+          v = *reinterpret_cast<const uint4*>(src + ch * 8);
+          v.x ^= flip;
+          v.y ^= flip;
+          v.z ^= flip;
+          v.w ^= flip;
         }
+        *reinterpret_cast<uint4*>(s_q + st * C::kTileBytes + (ch / 8) * C::kHalf + row * 128 +
+                                  (((ch % 8) ^ (row & 7)) << 4)) = v;
+      }
+      fence_async_shared();
+      mbar_arrive(&c.q_ready[st]);
+    };
+    AttnSegment s = attn_segment<kTile, kBlk>(p, at, w0, w_end);
+    StreamRange r = stream_range(p, at, s, st);
+    if (r.end > r.begin) load_q(at);
+    for (int w = w0; w < w_end;) {
+      const int rows = at.req.qlen * p.group, cached = at.req.seq - at.req.qlen;
+      const int fr = at.tile * kTile + st * kRowsPerStream + row;  // flattened row
+      const bool live = fr < rows;
+      const int t = fr / p.group, head = at.head * p.group + fr - t * p.group;
+      float m = -INFINITY, l = 0.f;
+      if (r.active) {
         // keys (j > low, j <= high) of this row, and of the stream's first and last row
         const int high = live ? cached + t : -1;
         const int low = p.window > 0 ? cached + t - p.window : -1;
@@ -387,7 +395,6 @@ __global__ void __launch_bounds__(kThreads, 1)
         const int high_min = cached + f_row / p.group;
         const int low_max =
             p.window > 0 ? cached + (min(f_row + kRowsPerStream, rows) - 1) / p.group - p.window : -1;
-        float m = -INFINITY, l = 0.f;
         for (int blk = r.begin; blk < r.end; ++blk) {
           mbar_wait_bounded(&c.s_full[st], s_phase, p.err, abort_flag);
           s_phase ^= 1u;
@@ -462,111 +469,113 @@ __global__ void __launch_bounds__(kThreads, 1)
           tc_fence_before();
           mbar_arrive(&c.p_ready[st]);
         }
-        if (r.end > r.begin) {
-          mbar_wait_bounded(&c.o_full[st], o_phase, p.err, abort_flag);
-          o_phase ^= 1u;
-          tc_fence_after();
-        }
-        bool final = s.whole;
-        int cs = 0, ce = -1;
-        if (!s.whole) {
-          cs = s.start / per;
-          ce = (s.end - 1) / per;
-          const int64_t slot = 2 * static_cast<int64_t>(blockIdx.x) + (blockIdx.x == cs ? 1 : 0);
-          // [D][256 rows]: the threads of a warp store neighbouring rows
-          float* po = p.partial_o + slot * (kTile * D) + st * kRowsPerStream + row;
-          if (r.end > r.begin) {
-#pragma unroll 1
-            for (int i = 0; i < D / 32; ++i) {
-              uint32_t o[32];
-              tmem_ld_32x32b_x32(t_o + i * 32, o);
-              tmem_ld_wait();
-#pragma unroll
-              for (int e = 0; e < 32; ++e) po[(i * 32 + e) * kTile] = __uint_as_float(o[e]);
-            }
-          }
-          float* pml = p.partial_ml + (slot * kTile + st * kRowsPerStream + row) * 2;
-          pml[0] = m;
-          pml[1] = l;  // 0: nothing seen, and perhaps no accumulator written
-          __threadfence();
-          stream_sync(st);
-          if (row == 0) {
-            int32_t* counter = p.counters + 2 * cs + st;
-            c.last[st] = atomicAdd(counter, 1) == ce - cs;
-            if (c.last[st]) *counter = 0;  // every other CTA of the item has arrived
-          }
-          stream_sync(st);
-          final = c.last[st] != 0;
-          if (final) __threadfence();
-        }
-        if (final) {
-          uint16_t* dst = p.out + (at.req.q0 + t) * p.out_token_stride + head * p.out_head_stride;
-          if (s.whole) {
-            const float inv = l != 0.f ? 1.f / l : 0.f;
-#pragma unroll 1
-            for (int i = 0; i < D / 32; ++i) {
-              uint32_t o[32];
-              if (r.end > r.begin) {
-                tmem_ld_32x32b_x32(t_o + i * 32, o);
-                tmem_ld_wait();
-              }
-              if (live) {
-#pragma unroll
-                for (int v = 0; v < 4; ++v) {
-                  uint32_t q[4];
-#pragma unroll
-                  for (int e = 0; e < 4; ++e)
-                    q[e] = l != 0.f ? pack_bf16x2(__uint_as_float(o[v * 8 + 2 * e]) * inv,
-                                                 __uint_as_float(o[v * 8 + 2 * e + 1]) * inv)
-                                   : 0u;
-                  *reinterpret_cast<uint4*>(dst + i * 32 + v * 8) = make_uint4(q[0], q[1], q[2], q[3]);
-                }
-              }
-            }
-          } else {
-            // partials of CTAs cs .. ce, in the order of the keys
-            m = -INFINITY;
-            l = 0.f;
-            for (int k = cs; k <= ce; ++k) {
-              const int64_t slot = 2 * static_cast<int64_t>(k) + (k == cs ? 1 : 0);
-              const float* pml = p.partial_ml + (slot * kTile + st * kRowsPerStream + row) * 2;
-              if (pml[1] != 0.f) m = fmaxf(m, pml[0]);
-            }
-            for (int k = cs; k <= ce; ++k) {
-              const int64_t slot = 2 * static_cast<int64_t>(k) + (k == cs ? 1 : 0);
-              const float* pml = p.partial_ml + (slot * kTile + st * kRowsPerStream + row) * 2;
-              if (pml[1] != 0.f) l += pml[1] * ex2(pml[0] - m);
-            }
-            const float inv = l != 0.f ? 1.f / l : 0.f;
-#pragma unroll 1
-            for (int i = 0; i < D / 8; ++i) {
-              float acc[8];
-#pragma unroll
-              for (int e = 0; e < 8; ++e) acc[e] = 0.f;
-              for (int k = cs; k <= ce; ++k) {
-                const int64_t slot = 2 * static_cast<int64_t>(k) + (k == cs ? 1 : 0);
-                const float* pml = p.partial_ml + (slot * kTile + st * kRowsPerStream + row) * 2;
-                if (pml[1] != 0.f) {
-                  const float f = ex2(pml[0] - m);
-                  const float* po = p.partial_o + slot * (kTile * D) + st * kRowsPerStream + row;
-#pragma unroll
-                  for (int e = 0; e < 8; ++e) acc[e] += f * po[(i * 8 + e) * kTile];
-                }
-              }
-              if (live)
-                *reinterpret_cast<uint4*>(dst + i * 8) =
-                    make_uint4(pack_bf16x2(acc[0] * inv, acc[1] * inv), pack_bf16x2(acc[2] * inv, acc[3] * inv),
-                               pack_bf16x2(acc[4] * inv, acc[5] * inv), pack_bf16x2(acc[6] * inv, acc[7] * inv));
-            }
-          }
-          if (live && p.lse != nullptr)
-            p.lse[static_cast<int64_t>(at.req.q0 + t) * p.q_heads + head] =
-                l != 0.f ? (m + log2f(l)) * 0.693147180559945309f : -INFINITY;
-        }
-        tc_fence_before();  // O is read before the next segment's P V overwrites it
       }
+      // The next segment's Q goes in before this one's results come out: S of this segment's last
+      // block is there, so its Q has been read.
+      const AttnCursor done = at;
+      const AttnSegment ds = s;
+      const StreamRange dr = r;
       w += s.units;
-      if (w < w_end) attn_advance<kTile>(p, at);
+      if (w < w_end) {
+        attn_advance<kTile>(p, at);
+        s = attn_segment<kTile, kBlk>(p, at, w, w_end);
+        r = stream_range(p, at, s, st);
+        if (r.end > r.begin) load_q(at);
+      }
+      if (!dr.active) continue;
+      const bool has_o = dr.end > dr.begin;
+      if (has_o) {
+        mbar_wait_bounded(&c.o_full[st], o_phase, p.err, abort_flag);
+        o_phase ^= 1u;
+        tc_fence_after();
+      }
+      bool final = ds.whole;
+      float total = l, scale = 1.f;
+      float o[D];
+#pragma unroll
+      for (int i = 0; i < D; ++i) o[i] = 0.f;
+      auto read_o = [&]() {
+#pragma unroll
+        for (int i = 0; i < D / 32; ++i) {
+          uint32_t v[32];
+          tmem_ld_32x32b_x32(t_o + i * 32, v);
+          tmem_ld_wait();
+#pragma unroll
+          for (int e = 0; e < 32; ++e) o[i * 32 + e] = __uint_as_float(v[e]);
+        }
+      };
+      if (has_o) read_o();
+      if (!ds.whole) {
+        const int cs = ds.start / per, ce = (ds.end - 1) / per, me = blockIdx.x;
+        // partial results lie as [D / 4][256 rows][4]: a warp's 16-byte pieces are neighbours
+        auto slot_of = [&](int k) { return 2 * static_cast<int64_t>(k) + (k == cs ? 1 : 0); };
+        auto o_of = [&](int k) {
+          return reinterpret_cast<float4*>(p.partial_o + slot_of(k) * (kTile * D)) + st * kRowsPerStream + row;
+        };
+        auto ml_of = [&](int k) {
+          return reinterpret_cast<float2*>(p.partial_ml) + slot_of(k) * kTile + st * kRowsPerStream + row;
+        };
+        if (has_o) {
+          float4* po = o_of(me);
+#pragma unroll
+          for (int i = 0; i < D / 4; ++i)
+            po[i * kTile] = make_float4(o[4 * i], o[4 * i + 1], o[4 * i + 2], o[4 * i + 3]);
+        }
+        *ml_of(me) = make_float2(m, l);  // a sum of 0: nothing seen, and perhaps no accumulator written
+        __threadfence();
+        stream_sync(st);
+        if (row == 0) {
+          int32_t* counter = p.counters + 2 * cs + st;
+          c.last[st] = atomicAdd(counter, 1) == ce - cs;
+          if (c.last[st]) *counter = 0;  // every other CTA of the item has arrived
+        }
+        stream_sync(st);
+        final = c.last[st] != 0;
+        if (final) {
+          // partials of CTAs cs .. ce, in the order of the keys whoever arrives last
+          __threadfence();
+          m = -INFINITY;
+#pragma unroll 4
+          for (int k = cs; k <= ce; ++k) {
+            const float2 ml = __ldcg(ml_of(k));
+            if (ml.y != 0.f) m = fmaxf(m, ml.x);
+          }
+          total = 0.f;
+#pragma unroll
+          for (int i = 0; i < D; ++i) o[i] = 0.f;
+          for (int k = cs; k <= ce; ++k) {
+            const float2 ml = __ldcg(ml_of(k));
+            if (ml.y == 0.f) continue;
+            const float f = ex2(ml.x - m);
+            total += f * ml.y;
+            const float4* po = o_of(k);
+#pragma unroll
+            for (int i = 0; i < D / 4; ++i) {
+              const float4 v = __ldcg(po + i * kTile);
+              o[4 * i] += f * v.x;
+              o[4 * i + 1] += f * v.y;
+              o[4 * i + 2] += f * v.z;
+              o[4 * i + 3] += f * v.w;
+            }
+          }
+        }
+      }
+      if (final && live) {
+        uint16_t* dst = p.out + (done.req.q0 + t) * p.out_token_stride + head * p.out_head_stride;
+        scale = total != 0.f ? 1.f / total : 0.f;
+#pragma unroll
+        for (int i = 0; i < D / 8; ++i) {
+          uint32_t q[4];
+#pragma unroll
+          for (int e = 0; e < 4; ++e)
+            q[e] = total != 0.f ? pack_bf16x2(o[8 * i + 2 * e] * scale, o[8 * i + 2 * e + 1] * scale) : 0u;
+          *reinterpret_cast<uint4*>(dst + i * 8) = make_uint4(q[0], q[1], q[2], q[3]);
+        }
+        if (p.lse != nullptr)
+          p.lse[static_cast<int64_t>(done.req.q0 + t) * p.q_heads + head] =
+              total != 0.f ? (m + log2f(total)) * 0.693147180559945309f : -INFINITY;
+      }
+      tc_fence_before();  // O is read before the next segment's P V overwrites it
     }
   }
   tc_fence_before();
