@@ -113,14 +113,21 @@ __global__ void __launch_bounds__(kThreads, 1)
     tma_prefetch_desc(&up.maps.k);
     tma_prefetch_desc(&up.maps.v);
   }
-  pdl_wait();
+  // Beside the tensor-core kernel of the same call, which touches other rows and another workspace:
+  // this one starts when all of that one's CTAs have started, so all earlier kernels are complete,
+  // and takes the SMs that it leaves. It waits for it at its end, so that whoever waits for this
+  // kernel has waited for both.
+  if (!up.beside) pdl_wait();
   pdl_trigger();
   attn_prefix<kTileRows, kBlock, kThreads>(p, s_prefix, s_warp);  // its barrier covers the inits too
   const int total = s_prefix[p.num_requests];
   const int per = (total + gridDim.x - 1) / gridDim.x;
   int w = blockIdx.x * per;
   const int w_end = min(total, w + per);
-  if (w >= w_end) return;  // the whole CTA
+  if (w >= w_end) {  // the whole CTA
+    pdl_wait();
+    return;
+  }
   AttnCursor at = attn_seek<kTileRows, kBlock>(p, s_prefix, w);
   volatile int* abort_flag = &c.abort_flag;
 
@@ -128,6 +135,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     const bool is_v = warp == kWarps + 1;
     attn_load_kv<D, kTileRows, S::kStages>(up, is_v, at, w, w_end, smem + (is_v ? S::kTile : 0), S::kStage, 0, 1,
                                            c.full, c.empty, abort_flag);
+    pdl_wait();
     return;
   }
   if (warp > kWarps) {
@@ -152,6 +160,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       if (w < w_end) attn_advance<kTileRows>(p, at);
     }
     cp_async_wait_all();  // nothing in flight into shared memory when the warp leaves
+    pdl_wait();
     return;
   }
 
@@ -406,6 +415,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     w += s.units;
     if (w < w_end) attn_advance<kTileRows>(p, at);
   }
+  pdl_wait();
 }
 
 int attn_ctas() {
@@ -420,14 +430,19 @@ int attn_ctas() {
   return cached[dev];
 }
 
-// The workspace: counters, then the partial sums and accumulators of 2 partials per CTA.
+// The workspace: for either kernel its counters, and the sums and accumulators of 2 partial results
+// per CTA (256 rows of the tensor-core kernel, 16 of the other).
 struct Workspace {
-  static constexpr int64_t kCounterBytes = 2 * kAttnMaxCtas * 4;
-  static int64_t ml_bytes() { return static_cast<int64_t>(2) * attn_ctas() * kAttnMaxPartialRows * 8; }
-  static int64_t o_bytes() {
-    return static_cast<int64_t>(2) * attn_ctas() * kAttnMaxPartialRows * 128 * 4;
+  static int64_t counters() { return 2 * kAttnMaxCtas * 4; }
+  static int64_t ml(int rows) { return static_cast<int64_t>(2) * attn_ctas() * rows * 8; }
+  static int64_t o(int rows) { return static_cast<int64_t>(2) * attn_ctas() * rows * 128 * 4; }
+  static int64_t part(int rows) { return counters() + ml(rows) + o(rows); }
+  static int64_t bytes() { return part(kAttnMaxPartialRows) + part(kTileRows); }
+  static void place(AttnParams* p, unsigned char* at, int rows) {
+    p->counters = reinterpret_cast<int32_t*>(at);
+    p->partial_ml = reinterpret_cast<float*>(at + counters());
+    p->partial_o = reinterpret_cast<float*>(at + counters() + ml(rows));
   }
-  static int64_t bytes() { return kCounterBytes + ml_bytes() + o_bytes(); }
 };
 
 // The cache as (values, then tokens and heads by growing stride, pages); boxes of box_rows tokens of
@@ -458,11 +473,12 @@ int cache_map(CUtensorMap* out, const void* base, const AttnParams& a, int head_
 }
 
 template <int D>
-int launch_rows(const AttnParams& a, const AttnMaps& maps, cudaStream_t s) {
+int launch_rows(const AttnParams& a, const AttnMaps& maps, bool beside, cudaStream_t s) {
   AttnLaunch p;
   p.a = a;
   p.maps = maps;
   p.negate_q = 0;
+  p.beside = beside;
   const size_t smem = RowsSmem<D>::kBytes + (static_cast<size_t>(a.num_requests) + 1) * 4;
   static bool done[64] = {false};
   int dev = 0;
@@ -551,9 +567,6 @@ extern "C" int lm_paged_attention(
   p.seq_lens = seq_lens;
   p.cu_q = cu_q;
   unsigned char* ws = static_cast<unsigned char*>(workspace);
-  p.counters = reinterpret_cast<int32_t*>(ws);
-  p.partial_ml = reinterpret_cast<float*>(ws + Workspace::kCounterBytes);
-  p.partial_o = reinterpret_cast<float*>(ws + Workspace::kCounterBytes + Workspace::ml_bytes());
   p.err = err_word;
   p.q_token_stride = q_token_stride;
   p.q_head_stride = q_head_stride;
@@ -587,11 +600,13 @@ extern "C" int lm_paged_attention(
   int rc = attn_make_maps(p, head_dim, &maps);
   if (rc) return rc;
   if (any_long) {
+    Workspace::place(&p, ws, kAttnMaxPartialRows);
     if (any_short) p.min_rows = kTileRows + 1;
     rc = attn_launch_umma(p, maps, head_dim, attn_ctas(), s);
     if (rc || !any_short) return rc;
     p.min_rows = 1;
     p.max_rows = kTileRows;
   }
-  return head_dim == 64 ? launch_rows<64>(p, maps, s) : launch_rows<128>(p, maps, s);
+  Workspace::place(&p, ws + Workspace::part(kAttnMaxPartialRows), kTileRows);
+  return head_dim == 64 ? launch_rows<64>(p, maps, any_long, s) : launch_rows<128>(p, maps, any_long, s);
 }

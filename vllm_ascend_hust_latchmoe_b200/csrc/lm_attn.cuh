@@ -220,6 +220,7 @@ struct AttnLaunch {
   AttnMaps maps;
   AttnParams a;
   int negate_q;
+  int beside;  // the kernel launched just before is the other half of the same call
 };
 
 int attn_make_maps(const AttnParams& a, int head_dim, AttnMaps* maps);

@@ -611,6 +611,7 @@ int attn_launch_umma(const AttnParams& a, const AttnMaps& maps, int head_dim, in
   AttnLaunch p;
   p.a = a;
   p.maps = maps;
+  p.beside = 0;
   // Q's sign takes a negative scale's, so that a row's largest S has its largest weight; with a
   // scale of 0 the masked scores (-inf) still have to vanish.
   p.negate_q = a.scale_log2 < 0.f;
