@@ -91,23 +91,44 @@ __device__ __forceinline__ int attn_tiles(const AttnParams& p, const AttnRequest
   return rows >= p.min_rows && rows <= p.max_rows ? (rows + TILE_ROWS - 1) / TILE_ROWS : 0;
 }
 
-// Exclusive prefix of the requests' costs in s_prefix[0 .. B]. Called by all NT threads.
+// Exclusive prefix of the requests' costs in s_prefix[0 .. B]. Called by all NT threads: a thread
+// takes a request, and the lanes of its warp share the tiles of one that has several.
 template <int TILE_ROWS, int BLOCK, int NT>
 __device__ __forceinline__ void attn_prefix(const AttnParams& p, int32_t* s_prefix, int32_t* s_warp) {
   const int B = p.num_requests;
   const int per = (B + NT - 1) / NT;
   const int b0 = threadIdx.x * per, b1 = min(B, b0 + per);
   int sum = 0;
-  for (int b = b0; b < b1; ++b) {
-    const AttnRequest r = attn_request(p, b, blockIdx.x == 0);
-    const int tiles = attn_tiles<TILE_ROWS>(p, r);
-    int cost = 0;
-    for (int t = 0; t < tiles; ++t) {
-      int lo, hi;
-      attn_tile_keys<TILE_ROWS>(p, r, t, lo, hi);
-      cost += attn_blocks<BLOCK>(lo, hi);
+  for (int i = 0; i < per; ++i) {
+    const int b = b0 + i;
+    AttnRequest r{0, 0, 0};
+    int tiles = 0, cost = 0;
+    if (b < b1) {
+      r = attn_request(p, b, blockIdx.x == 0);
+      tiles = attn_tiles<TILE_ROWS>(p, r);
     }
-    s_prefix[b + 1] = cost * p.kv_heads;
+    if (tiles == 1) {
+      int lo, hi;
+      attn_tile_keys<TILE_ROWS>(p, r, 0, lo, hi);
+      cost = attn_blocks<BLOCK>(lo, hi);
+    }
+    for (unsigned many = __ballot_sync(0xffffffffu, tiles > 1); many != 0; many &= many - 1) {
+      const int src = __ffs(many) - 1;
+      AttnRequest o;
+      o.q0 = 0;
+      o.qlen = __shfl_sync(0xffffffffu, r.qlen, src);
+      o.seq = __shfl_sync(0xffffffffu, r.seq, src);
+      const int n = __shfl_sync(0xffffffffu, tiles, src);
+      int part = 0;
+      for (int t = threadIdx.x & 31; t < n; t += 32) {
+        int lo, hi;
+        attn_tile_keys<TILE_ROWS>(p, o, t, lo, hi);
+        part += attn_blocks<BLOCK>(lo, hi);
+      }
+      part = __reduce_add_sync(0xffffffffu, part);
+      if ((threadIdx.x & 31) == src) cost = part;
+    }
+    if (b < b1) s_prefix[b + 1] = cost * p.kv_heads;
     sum += cost * p.kv_heads;
   }
   int incl = sum;
@@ -135,7 +156,7 @@ struct AttnCursor {
   int b, head, tile, tiles, off;
 };
 
-// The cursor at unit w (w < s_prefix[B]); every thread computes it alike.
+// The cursor at unit w (w < s_prefix[B]); every warp computes it alike.
 template <int TILE_ROWS, int BLOCK>
 __device__ __forceinline__ AttnCursor attn_seek(const AttnParams& p, const int32_t* s_prefix, int w) {
   int lo_b = 0, hi_b = p.num_requests;
@@ -151,12 +172,29 @@ __device__ __forceinline__ AttnCursor attn_seek(const AttnParams& p, const int32
   const int per_head = (s_prefix[lo_b + 1] - s_prefix[lo_b]) / p.kv_heads;
   c.head = c.off / per_head;
   c.off -= c.head * per_head;
-  for (c.tile = 0;; ++c.tile) {
-    int lo, hi;
-    attn_tile_keys<TILE_ROWS>(p, c.req, c.tile, lo, hi);
-    const int n = attn_blocks<BLOCK>(lo, hi);
-    if (c.off < n) break;
-    c.off -= n;
+  // the tile that unit `off` of the head falls into: a lane per tile, 32 tiles at a time
+  for (c.tile = 0; c.tiles > 1;) {
+    const int lane = threadIdx.x & 31, t = c.tile + lane;
+    int lo, hi, n = 0;
+    if (t < c.tiles) {
+      attn_tile_keys<TILE_ROWS>(p, c.req, t, lo, hi);
+      n = attn_blocks<BLOCK>(lo, hi);
+    }
+    int incl = n;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int u = __shfl_up_sync(0xffffffffu, incl, o);
+      if (lane >= o) incl += u;
+    }
+    const unsigned past = __ballot_sync(0xffffffffu, t < c.tiles && incl > c.off);
+    if (past != 0) {
+      const int at = __ffs(past) - 1;
+      c.off -= __shfl_sync(0xffffffffu, incl - n, at);
+      c.tile += at;
+      break;
+    }
+    c.off -= __shfl_sync(0xffffffffu, incl, 31);
+    c.tile += 32;
   }
   return c;
 }

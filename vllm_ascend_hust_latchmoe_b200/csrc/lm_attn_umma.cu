@@ -355,25 +355,35 @@ __global__ void __launch_bounds__(kThreads, 1)
     uint32_t s_phase = 0, o_phase = 0;
     // A wait that gave up is recorded and stops the loader and the MMA warp; the rows go on to the
     // end over whatever TMEM holds (every later wait returns at once), so that barriers match.
-    // this thread's row of a segment's Q into shared memory
+    // This warp's 32 rows of a segment's Q into shared memory, D / 8 lanes to a row, whose place in
+    // memory comes from the lane that the row belongs to.
     auto load_q = [&](const AttnCursor& q_at) {
+      constexpr int kLanes = D / 8, kRows = 32 / kLanes;  // per load
       const int fr = q_at.tile * kTile + st * kRowsPerStream + row;
       const int t = fr / p.group, head = q_at.head * p.group + fr - t * p.group;
-      const bool live = fr < q_at.req.qlen * p.group;
-      const uint16_t* src = p.q + (q_at.req.q0 + t) * p.q_token_stride + head * p.q_head_stride;
+      const int64_t off = (q_at.req.q0 + t) * p.q_token_stride + head * p.q_head_stride;
+      const unsigned live_rows = __ballot_sync(0xffffffffu, fr < q_at.req.qlen * p.group);
       const uint32_t flip = up.negate_q ? 0x80008000u : 0u;
+      const int ch = lane % kLanes;
+      unsigned char* dst = s_q + st * C::kTileBytes + (ch / 8) * C::kHalf;
+      uint4 v[32 / kRows];
 #pragma unroll
-      for (int ch = 0; ch < D / 8; ++ch) {
-        uint4 v = make_uint4(0, 0, 0, 0);
-        if (live) {
-          v = *reinterpret_cast<const uint4*>(src + ch * 8);
-          v.x ^= flip;
-          v.y ^= flip;
-          v.z ^= flip;
-          v.w ^= flip;
+      for (int i = 0; i < 32 / kRows; ++i) {
+        const int from = i * kRows + lane / kLanes;
+        const int64_t src = __shfl_sync(0xffffffffu, off, from);
+        v[i] = make_uint4(0, 0, 0, 0);
+        if ((live_rows >> from) & 1u) {
+          v[i] = *reinterpret_cast<const uint4*>(p.q + src + ch * 8);
+          v[i].x ^= flip;
+          v[i].y ^= flip;
+          v[i].z ^= flip;
+          v[i].w ^= flip;
         }
-        *reinterpret_cast<uint4*>(s_q + st * C::kTileBytes + (ch / 8) * C::kHalf + row * 128 +
-                                  (((ch % 8) ^ (row & 7)) << 4)) = v;
+      }
+#pragma unroll
+      for (int i = 0; i < 32 / kRows; ++i) {
+        const int q_row = (warp & 3) * 32 + i * kRows + lane / kLanes;
+        *reinterpret_cast<uint4*>(dst + q_row * 128 + (((ch % 8) ^ (q_row & 7)) << 4)) = v[i];
       }
       fence_async_shared();
       mbar_arrive(&c.q_ready[st]);
