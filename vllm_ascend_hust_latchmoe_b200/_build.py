@@ -1,8 +1,9 @@
 """Build liblatchmoe_b200.so in-tree with nvcc for sm_100a (B200).
 
 The library is a plain C-ABI shared object (no torch types cross its boundary); the
-package loads it with ctypes. It is built next to this file so that it travels with the
-source tree; nothing is installed into site-packages.
+package loads it with ctypes. ``_decoder_ops.so`` beside it is the decoder operators' Python
+binding (host code only: torch tensors in, calls of the C ABI out). Both are built next to
+this file so that they travel with the source tree; nothing is installed into site-packages.
 """
 
 from __future__ import annotations
@@ -10,6 +11,7 @@ from __future__ import annotations
 import os
 import shutil
 import subprocess
+import sysconfig
 from pathlib import Path
 
 PKG_DIR = Path(__file__).resolve().parent
@@ -18,6 +20,9 @@ CSRC = PKG_DIR / "csrc"
 INCLUDE = REPO_ROOT / "include"
 LIB_NAME = "liblatchmoe_b200.so"
 LIB_PATH = PKG_DIR / LIB_NAME
+
+BINDING_SRC = CSRC / "binding" / "decoder_ops.cpp"
+BINDING_PATH = PKG_DIR / "_decoder_ops.so"
 
 NVCC_FLAGS = (
     "-gencode",
@@ -47,18 +52,43 @@ def nvcc_path() -> str:
     raise RuntimeError("nvcc not found: set NVCC or put /usr/local/cuda/bin on PATH")
 
 
-def build(force: bool = False, verbose: bool = False) -> Path:
-    """Compile every .cu under csrc/ into one shared library (skipped when up to date)."""
-    if not force and LIB_PATH.exists() and LIB_PATH.stat().st_mtime >= _inputs_mtime():
-        return LIB_PATH
-    tmp = LIB_PATH.with_suffix(".so.tmp")
-    cmd = [nvcc_path(), *NVCC_FLAGS, f"-I{INCLUDE}", "-o", str(tmp), *map(str, _sources())]
+def _run(what: str, cmd: list[str], out: Path, verbose: bool) -> None:
     if verbose:
         print(" ".join(cmd), flush=True)
     proc = subprocess.run(cmd, capture_output=True, text=True)
     if proc.returncode != 0:
-        raise RuntimeError(f"nvcc failed ({proc.returncode}):\n{proc.stdout}\n{proc.stderr}")
-    os.replace(tmp, LIB_PATH)
+        raise RuntimeError(f"{what} failed ({proc.returncode}):\n{proc.stdout}\n{proc.stderr}")
+    os.replace(cmd[cmd.index("-o") + 1], out)
+
+
+def build_binding(force: bool = False, verbose: bool = False) -> Path:
+    """Compile the decoder operators' binding with the host compiler (skipped when up to date)."""
+    newest = max(p.stat().st_mtime for p in (BINDING_SRC, *INCLUDE.glob("*.h")))
+    if not force and BINDING_PATH.exists() and BINDING_PATH.stat().st_mtime >= newest:
+        return BINDING_PATH
+    import torch
+
+    root = Path(torch.__file__).resolve().parent
+    cuda = Path(nvcc_path()).resolve().parents[1]
+    cmd = [os.environ.get("CXX") or "g++", "-O2", "-std=c++17", "-shared", "-fPIC",
+           f"-D_GLIBCXX_USE_CXX11_ABI={int(torch.compiled_with_cxx11_abi())}", f"-I{INCLUDE}",
+           f"-I{root / 'include'}", f"-I{root / 'include/torch/csrc/api/include'}",
+           f"-I{sysconfig.get_paths()['include']}", f"-I{cuda / 'include'}",
+           "-o", str(BINDING_PATH.with_suffix(".so.tmp")), str(BINDING_SRC),
+           f"-L{root / 'lib'}", "-ltorch", "-ltorch_cpu", "-lc10", "-lc10_cuda", "-ltorch_python"]
+    _run("the binding's build", cmd, BINDING_PATH, verbose)
+    return BINDING_PATH
+
+
+def build(force: bool = False, verbose: bool = False) -> Path:
+    """Compile every .cu under csrc/ into one shared library, and the binding (each skipped
+    when up to date)."""
+    build_binding(force, verbose)
+    if not force and LIB_PATH.exists() and LIB_PATH.stat().st_mtime >= _inputs_mtime():
+        return LIB_PATH
+    tmp = LIB_PATH.with_suffix(".so.tmp")
+    _run("nvcc", [nvcc_path(), *NVCC_FLAGS, f"-I{INCLUDE}", "-o", str(tmp), *map(str, _sources())],
+         LIB_PATH, verbose)
     return LIB_PATH
 
 
