@@ -30,6 +30,7 @@ struct TableParams {
   int32_t* err;
   int64_t table_stride, max_tokens;
   int num_requests, page_size, max_pages, free_capacity;
+  int wide;  // positions and slots take 16-byte stores
 };
 
 // Exclusive prefix sums of two values per thread over the block; the totals come back too.
@@ -71,6 +72,62 @@ __device__ __forceinline__ void block_scan2(int64_t& a, int64_t& b, int64_t& tot
   b = ib - b + (warp ? s_warp[warp - 1][1] : 0);
 }
 
+// The last of n ascending values that is at most x (values[0] is).
+__device__ __forceinline__ int last_at_most(const int32_t* values, int n, int64_t x) {
+  int lo = 0, hi = n;
+  while (hi - lo > 1) {
+    const int mid = (lo + hi) >> 1;
+    if (values[mid] <= x) lo = mid; else hi = mid;
+  }
+  return lo;
+}
+
+// Positions and slots of N neighbouring tokens a thread, from the requests' first tokens (s_cu), pages
+// granted before them (s_page) and cached lengths (inverted: no place for the new tokens).
+template <int N>
+__device__ __forceinline__ void place_tokens(const TableParams& p, const int32_t* s_cu, const int32_t* s_page,
+                                             const int32_t* s_cached, int free_count, int tid, int stride) {
+  const int B = p.num_requests, page = p.page_size, total = s_cu[B];
+  for (int64_t t0 = static_cast<int64_t>(tid) * N; t0 < p.max_tokens; t0 += static_cast<int64_t>(stride) * N) {
+    int pos[N];
+    long long slot[N];
+    // the last request that starts at or before t0: the one that t0 belongs to
+    int lo = t0 < total ? last_at_most(s_cu, B, t0) : 0;
+#pragma unroll
+    for (int e = 0; e < N; ++e) {
+      const int64_t t = t0 + e;
+      pos[e] = 0;
+      slot[e] = -1;
+      if (t >= total) continue;
+      while (t >= s_cu[lo + 1]) ++lo;
+      const int kept = s_cached[lo], c = kept < 0 ? ~kept : kept;
+      pos[e] = c + static_cast<int>(t) - s_cu[lo];
+      if (kept < 0) continue;
+      const int have = (c + page - 1) / page, i = pos[e] / page;
+      // pages already held are read from the table, granted ones from the stack (another CTA may be
+      // writing their table entries)
+      const int id = i < have ? p.tables[lo * p.table_stride + i]
+                              : p.free_pages[free_count - 1 - (s_page[lo] + i - have)];
+      if (id >= 0)
+        slot[e] = static_cast<long long>(id) * page + (pos[e] - i * page);
+      else
+        record_error(p.err, LM_DEVERR_BAD_PAGE);
+    }
+    if (N == 4 && p.wide && t0 + N <= p.max_tokens) {
+      *reinterpret_cast<int4*>(p.positions + t0) = make_int4(pos[0], pos[1 % N], pos[2 % N], pos[3 % N]);
+      reinterpret_cast<longlong2*>(p.slots + t0)[0] = make_longlong2(slot[0], slot[1 % N]);
+      reinterpret_cast<longlong2*>(p.slots + t0)[1] = make_longlong2(slot[2 % N], slot[3 % N]);
+    } else {
+#pragma unroll
+      for (int e = 0; e < N; ++e) {
+        if (t0 + e >= p.max_tokens) break;
+        p.positions[t0 + e] = pos[e];
+        p.slots[t0 + e] = slot[e];
+      }
+    }
+  }
+}
+
 // Every CTA scans all requests (they fit one pass of its threads) and writes its share of the
 // tables and of the tokens. All reads of arrays that the call may overwrite in place (cached
 // lengths, the free count) come before the cluster's barrier, all writes to them after it.
@@ -83,8 +140,8 @@ __global__ void __launch_bounds__(kTableThreads) page_tables_kernel(const TableP
   if (threadIdx.x == 0) s_used = 0;
   const int B = p.num_requests, page = p.page_size;
   int32_t* s_cu = s_mem;               // [B + 1] first token of each request
-  int32_t* s_page = s_cu + B + 1;      // [B] pages granted before it, or -1: none for it
-  int32_t* s_cached = s_page + B;      // [B]
+  int32_t* s_page = s_cu + B + 1;      // [B] pages needed before it
+  int32_t* s_cached = s_page + B;      // [B] cached length; inverted where the request gets no place
   const int per = (B + kTableThreads - 1) / kTableThreads;
   int free_count = *p.free_count;
   if (free_count < 0 || free_count > p.free_capacity) {
@@ -130,14 +187,13 @@ __global__ void __launch_bounds__(kTableThreads) page_tables_kernel(const TableP
     const int b = threadIdx.x * per + i;
     if (i >= per || b >= B) continue;
     s_cu[b] = static_cast<int32_t>(min(at_fresh, p.max_tokens));
-    s_cached[b] = cached[i];
     bool ok = need[i] >= 0;
     if (ok && need[i] > 0 && at_need + need[i] > free_count) {
       record_error(p.err, LM_DEVERR_NO_PAGES);
       ok = false;
     }
-    // a request that needs no page may stand past the stack's end: it reads none
-    s_page[b] = ok ? static_cast<int32_t>(min(at_need, static_cast<int64_t>(free_count))) : -1;
+    s_page[b] = static_cast<int32_t>(min(at_need, static_cast<int64_t>(0x7fffffff)));
+    s_cached[b] = ok ? cached[i] : ~cached[i];
     if (ok && need[i] > 0) granted = static_cast<int>(at_need) + need[i];
     at_need += max(need[i], 0);
     at_fresh += fresh[i];
@@ -157,42 +213,21 @@ __global__ void __launch_bounds__(kTableThreads) page_tables_kernel(const TableP
   for (int b = tid; b <= B; b += stride) {
     p.cu_q[b] = s_cu[b];
     if (b == B) break;
-    const int c = s_cached[b], n = s_page[b] >= 0 ? s_cu[b + 1] - s_cu[b] : 0;
-    p.seq_lens[b] = c + n;
+    const int kept = s_cached[b];
+    p.seq_lens[b] = kept < 0 ? ~kept : kept + s_cu[b + 1] - s_cu[b];
   }
-  // new table entries: a warp per request
-  const int lane = threadIdx.x & 31;
-  for (int b = tid >> 5; b < B; b += stride >> 5) {
-    if (s_page[b] < 0) continue;
-    const int c = s_cached[b], n = s_cu[b + 1] - s_cu[b];
-    const int have = (c + page - 1) / page, total = (c + n + page - 1) / page;
-    for (int i = have + lane; i < total; i += 32)
-      p.tables[b * p.table_stride + i] = p.free_pages[free_count - 1 - (s_page[b] + i - have)];
+  // new table entries: a thread per granted page
+  for (int j = tid; j < s_used; j += stride) {
+    const int b = last_at_most(s_page, B, j);
+    const int have = (s_cached[b] + page - 1) / page;
+    p.tables[b * p.table_stride + have + j - s_page[b]] = p.free_pages[free_count - 1 - j];
   }
-  for (int64_t t = tid; t < p.max_tokens; t += stride) {
-    int pos = 0;
-    int64_t slot = -1;
-    if (t < total_fresh) {
-      int lo = 0, hi = B;  // last request that starts at or before t and is not empty
-      while (hi - lo > 1) {
-        const int mid = (lo + hi) >> 1;
-        if (s_cu[mid] <= t) lo = mid; else hi = mid;
-      }
-      const int c = s_cached[lo];
-      pos = c + static_cast<int>(t) - s_cu[lo];
-      if (s_page[lo] >= 0) {
-        const int have = (c + page - 1) / page, i = pos / page;
-        // pages already held are read from the table, granted ones from the stack (another CTA
-        // may be writing their table entries)
-        const int pg = i < have ? p.tables[lo * p.table_stride + i]
-                                : p.free_pages[free_count - 1 - (s_page[lo] + i - have)];
-        slot = pg < 0 ? -1 : static_cast<int64_t>(pg) * page + pos - i * page;
-        if (pg < 0) record_error(p.err, LM_DEVERR_BAD_PAGE);
-      }
-    }
-    p.positions[t] = pos;
-    p.slots[t] = slot;
-  }
+  // tokens: one a thread while that is enough, else 4 neighbours, with one search and their reads
+  // in flight together
+  if (p.max_tokens <= stride)
+    place_tokens<1>(p, s_cu, s_page, s_cached, free_count, tid, stride);
+  else
+    place_tokens<4>(p, s_cu, s_page, s_cached, free_count, tid, stride);
 }
 
 // One block: the pages of the listed rows go back onto the free stack in row order.
@@ -522,7 +557,8 @@ extern "C" int lm_build_page_tables(const int32_t* cached_lens, const int32_t* n
     return fail(LM_ERR_INVALID_ARGUMENT, "lm_build_page_tables: null pointer");
   const TableParams p{cached_lens, new_lens, block_tables, free_pages, free_count, free_count_out,
                       seq_lens, cu_q, positions, slot_mapping, err_word, table_stride, max_tokens,
-                      num_requests, page_size, max_pages, free_capacity};
+                      num_requests, page_size, max_pages, free_capacity,
+                      ((reinterpret_cast<uintptr_t>(positions) | reinterpret_cast<uintptr_t>(slot_mapping)) & 15) == 0};
   const size_t smem = (3 * static_cast<size_t>(num_requests) + 1) * 4;
   if (smem > 48 * 1024) {
     const int rc = check_cuda(cudaFuncSetAttribute(page_tables_kernel,
@@ -531,7 +567,7 @@ extern "C" int lm_build_page_tables(const int32_t* cached_lens, const int32_t* n
                               "lm_build_page_tables: smem attribute");
     if (rc) return rc;
   }
-  const int ctas = max_tokens <= 2 * kTableThreads && num_requests <= kTableThreads ? 1 : kTableCtas;
+  const int ctas = max_tokens <= 4 * kTableThreads && num_requests <= kTableThreads ? 1 : kTableCtas;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(ctas);
   cfg.blockDim = dim3(kTableThreads);
