@@ -31,11 +31,15 @@ struct UmmaCfg {
   static constexpr int kTileBytes = kHalf * (D / 64);   // a K, V or Q tile
   static constexpr int kStages = D == 128 ? 5 : 8;
   static constexpr int kSmem = (2 + kStages) * kTileBytes + 1024;
+  // With D = 64 a stream's 256 TMEM columns hold S (128), O (64) and P (64) side by side, so S of the
+  // next block is made while this block's weights are; with D = 128 P lies over S and S waits for P V.
+  static constexpr bool kOwnP = D == 64;
+  static constexpr int kColP = kOwnP ? 192 : 0;
 };
 
 struct Ctrl {
   uint64_t kv_full[8], kv_empty[8];
-  uint64_t q_ready[2], s_full[2], p_half[2], p_ready[2], o_full[2], turn[2];
+  uint64_t q_ready[2], s_full[2], s_read[2], p_half[2], p_ready[2], o_full[2], turn[2];
   uint32_t tmem_base;
   int abort_flag;
   int last[2];
@@ -189,6 +193,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     for (int i = 0; i < 2; ++i) {
       mbar_init(&c.q_ready[i], kRowsPerStream);
       mbar_init(&c.s_full[i], 1);
+      mbar_init(&c.s_read[i], kRowsPerStream);
       mbar_init(&c.p_half[i], kRowsPerStream);
       mbar_init(&c.p_ready[i], kRowsPerStream);
       mbar_init(&c.o_full[i], 1);
@@ -293,10 +298,18 @@ __global__ void __launch_bounds__(kThreads, 1)
           ok = warp_wait(&c.kv_full[stage], kv_phase, p.err, abort_flag);  // K arrives after V
           if (!ok) break;
         }
+        const bool next = blk + 1 >= r.begin && blk + 1 < r.end;
+        if constexpr (C::kOwnP) {  // S of the next block as soon as this one's has been read
+          if (mine) ok = warp_wait(&c.s_read[st], p_phase, p.err, abort_flag);
+          if (!ok) break;
+          if (next) issue_s(stage);
+          if (blk + 1 < s.blk1) release(stage, next);
+        }
         ok = warp_wait(&c.kv_full[v_tile], v_phase, p.err, abort_flag);
         if (!ok) break;
         // The streams take turns, so that one's softmax runs beside the other's MMAs; left alone they
-        // fall into step, and exponentials and MMAs wait for their own kind (1027 against 930 us).
+        // fall into step, and exponentials and MMAs wait for their own kind (4096-token chunk over
+        // 16384 keys: 1027 against 909 us when it was tried, and 681 against 588 us with D = 64).
         ok = warp_wait(&c.turn[st], turn_phase, p.err, abort_flag);
         if (!ok) break;
         turn_phase ^= 1u;
@@ -325,20 +338,19 @@ __global__ void __launch_bounds__(kThreads, 1)
             if (elect_one()) {
 #pragma unroll
               for (int k = part * kBlk / 32; k < (part + 1) * kBlk / 32; ++k)
-                umma_bf16_ts(t_o, t_s + k * 8, v_desc + k * (2048 >> 4), idesc_o, k > 0 ? 1u : accumulate);
-              if (part == 1 && blk == r.end - 1) umma_commit(&c.o_full[st]);
+                umma_bf16_ts(t_o, t_s + C::kColP + k * 8, v_desc + k * (2048 >> 4), idesc_o, k > 0 ? 1u : accumulate);
+              if (part == 1 && (C::kOwnP || blk == r.end - 1)) umma_commit(&c.o_full[st]);
             }
             __syncwarp();
           }
           if (!ok) break;
           p_phase ^= 1u;
         }
-        const bool next = blk + 1 >= r.begin && blk + 1 < r.end;
-        if (next) issue_s(stage);
+        if (!C::kOwnP && next) issue_s(stage);
         if (elect_one()) mbar_arrive(&c.turn[1 - st]);
         release(v_tile, mine);
         if (blk + 1 < s.blk1) {
-          release(stage, next);
+          if (!C::kOwnP) release(stage, next);
           next_stage();
         }
       }
@@ -413,6 +425,10 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll
           for (int i = 0; i < 4; ++i) tmem_ld_32x32b_x32(t_s + i * 32, x[i]);
           tmem_ld_wait();
+          if constexpr (C::kOwnP) {
+            tc_fence_before();
+            mbar_arrive(&c.s_read[st]);
+          }
           const int j0 = blk * kBlk;
           if (j0 + kBlk - 1 > high_min || j0 <= low_max) {
 #pragma unroll
@@ -433,6 +449,13 @@ __global__ void __launch_bounds__(kThreads, 1)
           }
           const float mx = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])) * p.scale_log2;
           const bool move = mx > m + kRescaleAbove || (m == -INFINITY && mx > m);
+          if constexpr (C::kOwnP) {
+            if (blk > r.begin) {  // P V of the last block: O is whole, P may be written again
+              mbar_wait_bounded(&c.o_full[st], o_phase, p.err, abort_flag);
+              o_phase ^= 1u;
+              tc_fence_after();
+            }
+          }
           if (__any_sync(0xffffffffu, move)) {
             const float nm = move ? mx : m;
             const float f = move ? (m == -INFINITY ? 0.f : ex2(m - nm)) : 1.f;
@@ -465,7 +488,7 @@ __global__ void __launch_bounds__(kThreads, 1)
               sum2 = add2(sum2, pair(a, b));
               packed[e] = pack_bf16x2(a, b);
             }
-            tmem_st_32x32b_x16(t_s + i * 16, packed);
+            tmem_st_32x32b_x16(t_s + C::kColP + i * 16, packed);
             if (i == 1) {  // P V may begin with the first half of the keys
               tmem_st_wait();
               tc_fence_before();
