@@ -550,8 +550,11 @@ int lm_rope_cache_write(const uint16_t* qkv, int64_t qkv_stride, const int32_t* 
  * cu_q[b] .. cu_q[b + 1] and the last of them stands at position seq_lens[b] - 1. A query at
  * position p sees key j when j <= p and (window == 0 or j > p - window). out [T][q heads]
  * [head_dim] bf16; lse [T][q heads] fp32 (may be NULL) = ln of the sum of exp(scale * q.k). A query
- * that sees no key gives zeros and an lse of -inf; tokens of no request are not written. Keys that
- * no query of a row tile sees are not read (stale cache contents, NaN included, do not matter).
+ * that sees no key gives zeros and an lse of -inf; tokens of no request are not written. What the
+ * cache holds past a sequence, before its window and in other pages does not matter, NaN included
+ * (a NaN or infinity in a V row that a request sees may reach the request's other queries of the
+ * same step). The softmax weights are rounded to bf16 for the product with V, sums and statistics
+ * are fp32.
  * head_dim 64 or 128, page_size a multiple of 16, num_q_heads a multiple of num_kv_heads, at most
  * 4096 requests; bases 16-byte aligned, strides multiples of 8 elements. max_q_len only chooses
  * kernels; results do not depend on it being right. The workspace

@@ -98,3 +98,14 @@ def test_cpu_tensors_are_refused():
     with pytest.raises(ValueError, match="CUDA"):
         ops.paged_attention(x.view(2, 1, 64), kc, kc, torch.zeros(1, 2), torch.zeros(1), torch.zeros(2),
                             x.view(2, 1, 64), max_q_len=1, workspace=torch.zeros(1))
+
+
+def test_sizes_past_the_counters_are_refused():
+    lib = _lib.load()
+    rc = lib.lm_add_rms_norm(FAKE, 64, None, 0, FAKE, 1e-6, 1 << 30, 64, None, 0, FAKE, 64, None, 64, None, 0, None)
+    _refused(rc, b"2^30")
+    # 2^22 single-token requests' rows over 2^24-token rows of the block table: more units than 32 bits count
+    rc = lib.lm_paged_attention(FAKE, 256, 64, FAKE, 2048, 128, 64, FAKE, 2048, 128, 64, 4, 16, FAKE, 1 << 20,
+                                1 << 20, FAKE, FAKE, 1, 1 << 24, 4, 2, 64, 1, 0.125, 0, FAKE, 256, 64, None, FAKE,
+                                1 << 40, None, None)
+    _refused(rc, b"too much work")

@@ -543,6 +543,14 @@ extern "C" int lm_paged_attention(
     return fail(LM_ERR_INVALID_ARGUMENT, "lm_paged_attention: bad sizes (at most 4096 requests)");
   if (num_requests == 0 || num_tokens == 0) return LM_OK;
   if (num_pages == 0) return fail(LM_ERR_INVALID_ARGUMENT, "lm_paged_attention: an empty cache");
+  {  // the launches count their units (row tiles x key blocks) in 32 bits
+    const bool small = static_cast<int64_t>(max_q_len) * (num_q_heads / num_kv_heads) <= kTileRows;
+    const int64_t tiles = num_tokens * num_q_heads / (small ? kTileRows : 2 * 128) +
+                          static_cast<int64_t>(num_requests) * num_kv_heads;
+    const int64_t blocks = (static_cast<int64_t>(max_pages) * page_size + kBlock - 1) / kBlock + 1;
+    if (tiles > 0x7fffffff / blocks)
+      return fail(LM_ERR_UNSUPPORTED, "lm_paged_attention: too much work for one call");
+  }
   if (q == nullptr || k_cache == nullptr || v_cache == nullptr || block_tables == nullptr ||
       seq_lens == nullptr || cu_q == nullptr || out == nullptr || workspace == nullptr)
     return fail(LM_ERR_INVALID_ARGUMENT, "lm_paged_attention: null pointer");

@@ -268,9 +268,9 @@ extern "C" int lm_add_rms_norm(const uint16_t* x, int64_t x_stride, const uint16
                                int64_t residual_out_stride, uint16_t* y, int64_t y_stride,
                                uint8_t* y8, int64_t y8_stride, float* scales, int32_t group_size,
                                void* stream) {
-  if (hidden_size <= 0 || hidden_size > kMaxHidden || num_tokens < 0 || num_tokens > 0x7fffffff)
+  if (hidden_size <= 0 || hidden_size > kMaxHidden || num_tokens < 0 || num_tokens > 0x3fffffff)
     return fail(LM_ERR_INVALID_ARGUMENT,
-                "lm_add_rms_norm: need 1 <= hidden_size <= 16384 and 0 <= num_tokens < 2^31");
+                "lm_add_rms_norm: need 1 <= hidden_size <= 16384 and 0 <= num_tokens < 2^30");
   if ((y == nullptr) == (y8 == nullptr) && num_tokens > 0)
     return fail(LM_ERR_INVALID_ARGUMENT, "lm_add_rms_norm: give one of y and y8");
   if (y8 != nullptr && (scales == nullptr || group_size < 0 ||

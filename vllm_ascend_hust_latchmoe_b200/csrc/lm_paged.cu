@@ -131,6 +131,8 @@ __device__ __forceinline__ void place_tokens(const TableParams& p, const int32_t
 // Every CTA scans all requests (they fit one pass of its threads) and writes its share of the
 // tables and of the tokens. All reads of arrays that the call may overwrite in place (cached
 // lengths, the free count) come before the cluster's barrier, all writes to them after it.
+// Latency-bound: 4.2 us a call for 64 requests with a token each, 9.2 us for 1021 requests with 30,000
+// tokens (replayed from a graph; 20.6 us when a request's pages were one warp's).
 __global__ void __launch_bounds__(kTableThreads) page_tables_kernel(const TableParams p) {
   pdl_wait();
   pdl_trigger();
