@@ -638,3 +638,11 @@ def test_refusals(cuda):
         ops.build_page_tables(**{**tab, "cached_lens": many, "new_lens": many, "seq_lens": many,
                                  "cu_q": torch.zeros(4098, **i32), "block_tables": torch.zeros(4097, 1, **i32)})
     assert _lib.DEVERR_NAMES[5]
+
+
+@pytest.mark.parametrize("T,Hq,Hkv,D,R,inter,norm", [(2049, 40, 8, 64, 64, False, True),
+                                                     (2048, 33, 11, 128, 64, True, False),
+                                                     (2500, 9, 3, 128, 128, False, False)])
+def test_rope_cache_write_of_many_tokens(cuda, T, Hq, Hkv, D, R, inter, norm):
+    """Sizes at which a warp takes several groups of query heads, the last of them ragged."""
+    test_rope_cache_write(cuda, T, Hq, Hkv, D, R, 16, inter, norm, "split")

@@ -322,10 +322,11 @@ __device__ __forceinline__ int rope_position(const RopeParams& p, int pos) {
 // heads' loads are in flight together. A lane's partners are its own neighbours (interleaved) or
 // the 8 values of the lane half / 8 away, which come by shuffle as the bf16 pairs they are. Needs
 // 8 | rot_dim, and 16 | rot_dim for pairs half a rotation apart. Measured at 4096 tokens x 40 heads
-// of 128 with norms: 21.5 us (4.0 TB/s, 62 % of the copy rate); instruction issue bounds it more
-// than memory does (26.6 us with twice the instructions per head; without norms 18.0 us). 2 or 8
-// heads in flight per lane measured 24.7 and 21.7 us, more registers or more blocks per SM 23.7
-// and 26.7 us. 16 tokens take 3.2 us.
+// of 128 with norms: 18.5 us (4.6 TB/s, 72 % of the copy rate); instruction issue bounds it more
+// than memory does (a version with 213 instructions per 32 lanes took 26.6 us, one with 156 21.5 us).
+// With one group of heads a warp, 2 or 8 heads in flight per lane measured 24.7 and 21.7 us in the
+// place of 21.5, more registers or more blocks per SM 23.7 and 26.7 us; the next group's loads ahead of
+// this one's arithmetic spill (20.6 us). 16 tokens take 3.2 us.
 constexpr int kRopeUnroll = 4;
 
 __device__ __forceinline__ void unpack8(const uint4& v, float (&f)[8]) {
@@ -340,12 +341,18 @@ __host__ __device__ constexpr int rope_heads_per_warp() {
   return kRopeUnroll * 32 / (D / 8);
 }
 
-template <int D>
+// Q chunks that a warp takes one after the other, with the rotation and weight in registers. Many
+// tokens fill the GPU anyway (4096 x 40 heads: 18.5 us with 4 against 21.5 with 1); few tokens wait
+// for one warp's chain (16: 6.8 against 3.2 us).
+constexpr int kRopeLoops = 4;
+constexpr int64_t kRopeManyTokens = 2048;
+
+template <int D, int LOOPS>
 __global__ void __launch_bounds__(kRopeWarps * 32, 4) rope_write_kernel(const RopeParams p) {
   constexpr int LANES = D / 8, HEADS = 32 / LANES, PER_WARP = rope_heads_per_warp<D>();
   const int lane = threadIdx.x & 31;
   const int64_t t = static_cast<int64_t>(blockIdx.x) * kRopeWarps + (threadIdx.x >> 5);
-  const int q_chunks = (p.q_heads + PER_WARP - 1) / PER_WARP;
+  const int q_chunks = (p.q_heads + PER_WARP * LOOPS - 1) / (PER_WARP * LOOPS);
   const int k_chunks = (p.kv_heads + PER_WARP - 1) / PER_WARP;
   pdl_wait();
   pdl_trigger();
@@ -355,7 +362,8 @@ __global__ void __launch_bounds__(kRopeWarps * 32, 4) rope_write_kernel(const Ro
   chunk -= kind == 0 ? 0 : kind == 1 ? q_chunks : q_chunks + k_chunks;
   const int heads = kind == 0 ? p.q_heads : p.kv_heads;  // of this kind
   const int first_head = kind == 0 ? 0 : kind == 1 ? p.q_heads : p.q_heads + p.kv_heads;
-  const int h0 = chunk * PER_WARP + lane / LANES;
+  if (kind == 0) chunk *= LOOPS;
+  int h0 = chunk * PER_WARP + lane / LANES;
   const int c0 = (lane % LANES) * 8;  // this lane's values of a head
 
   // the position first: the cosines' addresses wait for it while the heads arrive
@@ -438,41 +446,50 @@ __global__ void __launch_bounds__(kRopeWarps * 32, 4) rope_write_kernel(const Ro
     }
   }
 
+  for (int left = kind == 0 ? LOOPS : 1;;) {
 #pragma unroll
-  for (int u = 0; u < kRopeUnroll; ++u) {
-    if (chunk * PER_WARP + u * HEADS >= heads) break;  // the same in the whole warp
-    float z[8], other[8];
-    unpack8(raw[u], z);
-    float r = 1.f;
-    if (weight != nullptr) {
-      float ss = 0.f;
+    for (int u = 0; u < kRopeUnroll; ++u) {
+      if (chunk * PER_WARP + u * HEADS >= heads) break;  // the same in the whole warp
+      float z[8], other[8];
+      unpack8(raw[u], z);
+      float r = 1.f;
+      if (weight != nullptr) {
+        float ss = 0.f;
 #pragma unroll
-      for (int e = 0; e < 8; ++e) ss += z[e] * z[e];
+        for (int e = 0; e < 8; ++e) ss += z[e] * z[e];
 #pragma unroll
-      for (int o = LANES / 2; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
-      r = rsqrtf(ss * (1.f / D) + p.eps);
+        for (int o = LANES / 2; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
+        r = rsqrtf(ss * (1.f / D) + p.eps);
+      }
+      if (p.interleaved) {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) other[e] = z[e ^ 1];
+      } else {
+        uint4 o;
+        o.x = __shfl_sync(0xffffffffu, raw[u].x, partner);
+        o.y = __shfl_sync(0xffffffffu, raw[u].y, partner);
+        o.z = __shfl_sync(0xffffffffu, raw[u].z, partner);
+        o.w = __shfl_sync(0xffffffffu, raw[u].w, partner);
+        unpack8(o, other);
+      }
+      // outside the rotation a value passes as it is: an infinity times a factor of 0 would not
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        const float turned = turns ? fmaf(other[e], b[e], z[e] * a[e]) : z[e] * a[e];
+        z[e] = weight != nullptr ? r * turned : turned;
+      }
+      if (h0 + u * HEADS < heads)
+        *reinterpret_cast<uint4*>(dst + u * head_stride) =
+            make_uint4(pack_bf16x2(z[0], z[1]), pack_bf16x2(z[2], z[3]), pack_bf16x2(z[4], z[5]),
+                       pack_bf16x2(z[6], z[7]));
     }
-    if (p.interleaved) {
+    if (LOOPS == 1 || --left == 0 || ++chunk * PER_WARP >= heads) return;
+    h0 += PER_WARP;
+    src += PER_WARP * D;
+    dst += kRopeUnroll * head_stride;
 #pragma unroll
-      for (int e = 0; e < 8; ++e) other[e] = z[e ^ 1];
-    } else {
-      uint4 o;
-      o.x = __shfl_sync(0xffffffffu, raw[u].x, partner);
-      o.y = __shfl_sync(0xffffffffu, raw[u].y, partner);
-      o.z = __shfl_sync(0xffffffffu, raw[u].z, partner);
-      o.w = __shfl_sync(0xffffffffu, raw[u].w, partner);
-      unpack8(o, other);
-    }
-    // outside the rotation a value passes as it is: an infinity times a factor of 0 would not
-#pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      const float turned = turns ? fmaf(other[e], b[e], z[e] * a[e]) : z[e] * a[e];
-      z[e] = weight != nullptr ? r * turned : turned;
-    }
-    if (h0 + u * HEADS < heads)
-      *reinterpret_cast<uint4*>(dst + u * head_stride) =
-          make_uint4(pack_bf16x2(z[0], z[1]), pack_bf16x2(z[2], z[3]), pack_bf16x2(z[4], z[5]),
-                     pack_bf16x2(z[6], z[7]));
+    for (int u = 0; u < kRopeUnroll; ++u)
+      if (h0 + u * HEADS < heads) raw[u] = *reinterpret_cast<const uint4*>(src + u * HEADS * D);
   }
 }
 
@@ -644,20 +661,23 @@ extern "C" int lm_rope_cache_write(
                      v_head_stride, num_tokens, num_pages * page_size, eps, num_q_heads,
                      num_kv_heads, rot_dim, max_positions, page_size, interleaved};
   // Pieces of 8 values where the rotation is made of them, else (an odd rot_dim, a table or weights
-  // that no 16-byte load fits) a warp per head: 21.5 against 52 us at 4096 tokens x 40 heads of 128.
+  // that no 16-byte load fits) a warp per head: 18.5 against 52 us at 4096 tokens x 40 heads of 128.
   const bool wide = rot_dim % (interleaved ? 8 : 16) == 0 &&
                     ((reinterpret_cast<uintptr_t>(cos_sin) | reinterpret_cast<uintptr_t>(q_norm_weight) |
                       reinterpret_cast<uintptr_t>(k_norm_weight)) & 15) == 0;
   const int per_warp = head_dim == 64 ? rope_heads_per_warp<64>() : rope_heads_per_warp<128>();
-  const int chunks = wide ? (num_q_heads + per_warp - 1) / per_warp +
+  const int loops = num_tokens >= kRopeManyTokens && num_q_heads > per_warp ? kRopeLoops : 1;
+  const int chunks = wide ? (num_q_heads + per_warp * loops - 1) / (per_warp * loops) +
                                 2 * ((num_kv_heads + per_warp - 1) / per_warp)
                           : 1;
   const int64_t units = wide ? num_tokens : num_tokens * heads;
   const int64_t blocks = (units + kRopeWarps - 1) / kRopeWarps;
   if (blocks > 0x7fffffff || chunks > 65535)
     return fail(LM_ERR_INVALID_ARGUMENT, "lm_rope_cache_write: too many tokens or heads");
-  auto kernel = head_dim == 64 ? (wide ? rope_write_kernel<64> : rope_write_any_kernel<64>)
-                               : (wide ? rope_write_kernel<128> : rope_write_any_kernel<128>);
+  auto kernel = head_dim == 64 ? rope_write_any_kernel<64> : rope_write_any_kernel<128>;
+  if (wide && loops == 1) kernel = head_dim == 64 ? rope_write_kernel<64, 1> : rope_write_kernel<128, 1>;
+  if (wide && loops > 1)
+    kernel = head_dim == 64 ? rope_write_kernel<64, kRopeLoops> : rope_write_kernel<128, kRopeLoops>;
   return check_cuda(launch_dependent(kernel, dim3(static_cast<unsigned>(blocks), chunks),
                                      dim3(kRopeWarps * 32), 0, static_cast<cudaStream_t>(stream), p),
                     "lm_rope_cache_write");
