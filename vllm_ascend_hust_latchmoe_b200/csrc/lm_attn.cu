@@ -601,9 +601,16 @@ extern "C" int lm_paged_attention(
   p.max_rows = 0x7fffffff;
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   // Requests of up to 16 rows per kv head read K and V for one small tile: the row kernel. More
-  // rows go to the tensor-core kernel. With what the host knows, one launch is often enough.
+  // rows go to the tensor-core kernel. A call with both kinds makes both launches, unless its short
+  // requests can only be a little work (by the block table's width, all of them single tokens): the
+  // tensor-core kernel takes 1.9 us for a block of keys and the row kernel 1.4, but a second launch
+  // costs 3 to 5 us (a 512-token chunk beside 7 single tokens over 4000 keys: 49 against 59 us in two
+  // launches, beside 15 of them 65 against 70).
   const bool any_long = static_cast<int64_t>(max_q_len) * p.group > kTileRows;
-  const bool any_short = p.group <= kTileRows && num_requests > 1;
+  const int64_t short_units = static_cast<int64_t>(num_requests) * num_kv_heads *
+                              ((static_cast<int64_t>(max_pages) * page_size + kBlock - 1) / kBlock);
+  const bool any_short = p.group <= kTileRows && num_requests > 1 &&
+                         short_units > 16 * static_cast<int64_t>(attn_ctas());
   AttnMaps maps;
   int rc = attn_make_maps(p, head_dim, &maps);
   if (rc) return rc;

@@ -559,7 +559,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         auto ml_of = [&](int k) {
           return reinterpret_cast<float2*>(p.partial_ml) + slot_of(k) * kTile + st * kRowsPerStream + row;
         };
-        if (has_o) {
+        if (has_o && live) {
           float4* po = o_of(me);
 #pragma unroll
           for (int i = 0; i < D / 4; ++i)
@@ -575,7 +575,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
         stream_sync(st);
         final = c.last[st] != 0;
-        if (final) {
+        if (final && live) {
           // partials of CTAs cs .. ce, in the order of the keys whoever arrives last
           __threadfence();
           m = -INFINITY;
