@@ -646,3 +646,23 @@ def test_refusals(cuda):
 def test_rope_cache_write_of_many_tokens(cuda, T, Hq, Hkv, D, R, inter, norm):
     """Sizes at which a warp takes several groups of query heads, the last of them ragged."""
     test_rope_cache_write(cuda, T, Hq, Hkv, D, R, 16, inter, norm, "split")
+
+
+@pytest.mark.parametrize("D", [64, 128])
+def test_attention_negative_scale(cuda, D):
+    """A scale's sign may stand in the queries: the same bits."""
+    g = _gen(cuda, D)
+    kc, vc = _bf16(g, 40, 16, 2, D), _bf16(g, 40, 16, 2, D)
+    tables = torch.randperm(40, device=cuda, generator=g).to(torch.int32).view(2, 20)
+    ws = ops.attention_workspace(cuda)
+    for new in ([1, 1], [300, 70]):
+        cu = torch.tensor([0, new[0], sum(new)], dtype=torch.int32, device=cuda)
+        seq = torch.tensor([310, 150], dtype=torch.int32, device=cuda)
+        q = _bf16(g, sum(new), 8, D)
+        outs = []
+        for sign in (1, -1):
+            out, lse = torch.empty_like(q), torch.empty(sum(new), 8, device=cuda)
+            ops.paged_attention(q * sign, kc, vc, tables, seq, cu, out, max_q_len=max(new), workspace=ws,
+                                scale=0.15 * sign, lse=lse)
+            outs.append((out, lse))
+        assert torch.equal(outs[0][0], outs[1][0]) and torch.equal(outs[0][1], outs[1][1])

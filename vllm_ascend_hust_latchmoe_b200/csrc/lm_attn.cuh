@@ -91,14 +91,16 @@ __device__ __forceinline__ int attn_tiles(const AttnParams& p, const AttnRequest
   return rows >= p.min_rows && rows <= p.max_rows ? (rows + TILE_ROWS - 1) / TILE_ROWS : 0;
 }
 
-// Exclusive prefix of the requests' costs in s_prefix[0 .. B]. Called by all NT threads: a thread
+// Exclusive prefix of the requests' costs in s_prefix[0 .. B], and the longest item's blocks (into
+// *s_longest, zeroed by the caller ahead of a barrier). Called by all NT threads: a thread
 // takes a request, and the lanes of its warp share the tiles of one that has several.
 template <int TILE_ROWS, int BLOCK, int NT>
-__device__ __forceinline__ void attn_prefix(const AttnParams& p, int32_t* s_prefix, int32_t* s_warp) {
+__device__ __forceinline__ void attn_prefix(const AttnParams& p, int32_t* s_prefix, int32_t* s_warp,
+                                            int* s_longest = nullptr) {
   const int B = p.num_requests;
   const int per = (B + NT - 1) / NT;
   const int b0 = threadIdx.x * per, b1 = min(B, b0 + per);
-  int sum = 0;
+  int sum = 0, longest = 0;
   for (int i = 0; i < per; ++i) {
     const int b = b0 + i;
     AttnRequest r{0, 0, 0};
@@ -111,6 +113,7 @@ __device__ __forceinline__ void attn_prefix(const AttnParams& p, int32_t* s_pref
       int lo, hi;
       attn_tile_keys<TILE_ROWS>(p, r, 0, lo, hi);
       cost = attn_blocks<BLOCK>(lo, hi);
+      longest = max(longest, cost);
     }
     for (unsigned many = __ballot_sync(0xffffffffu, tiles > 1); many != 0; many &= many - 1) {
       const int src = __ffs(many) - 1;
@@ -123,7 +126,9 @@ __device__ __forceinline__ void attn_prefix(const AttnParams& p, int32_t* s_pref
       for (int t = threadIdx.x & 31; t < n; t += 32) {
         int lo, hi;
         attn_tile_keys<TILE_ROWS>(p, o, t, lo, hi);
-        part += attn_blocks<BLOCK>(lo, hi);
+        const int n_blocks = attn_blocks<BLOCK>(lo, hi);
+        part += n_blocks;
+        longest = max(longest, n_blocks);
       }
       part = __reduce_add_sync(0xffffffffu, part);
       if ((threadIdx.x & 31) == src) cost = part;
@@ -139,6 +144,7 @@ __device__ __forceinline__ void attn_prefix(const AttnParams& p, int32_t* s_pref
     if (lane >= o) incl += u;
   }
   if (lane == 31) s_warp[warp] = incl;
+  if (s_longest != nullptr) atomicMax(s_longest, longest);
   __syncthreads();
   int base = incl - sum;
   for (int w = 0; w < warp; ++w) base += s_warp[w];

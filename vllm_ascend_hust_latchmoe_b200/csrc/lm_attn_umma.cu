@@ -190,6 +190,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   extern __shared__ unsigned char smem_raw[];
   __shared__ Ctrl c;
   __shared__ int32_t s_warp[kThreads / 32];
+  __shared__ int s_longest;
   unsigned char* smem = reinterpret_cast<unsigned char*>(
       (reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~static_cast<uintptr_t>(1023));
   unsigned char* s_q = smem;                       // [2][kTileBytes]
@@ -211,6 +212,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       mbar_init(&c.turn[i], 1);
     }
     c.abort_flag = 0;
+    s_longest = 0;
     fence_mbarrier_init();
   }
   if (warp == 9 && lane == 0) {
@@ -221,9 +223,14 @@ __global__ void __launch_bounds__(kThreads, 1)
   pdl_trigger();
   // the prefix lies where Q goes later
   int32_t* s_prefix = reinterpret_cast<int32_t*>(s_q);
-  attn_prefix<kTile, kBlk, kThreads>(p, s_prefix, s_warp);
+  __syncthreads();  // s_longest
+  attn_prefix<kTile, kBlk, kThreads>(p, s_prefix, s_warp, &s_longest);
   const int total = s_prefix[p.num_requests];
-  const int per = (total + gridDim.x - 1) / gridDim.x;
+  // A few long items are not cut into more pieces than pay: a block takes 1.9 us, another piece to
+  // merge about as much, so n blocks are best cut into sqrt(n) pieces (16 items of 17 blocks: 42 us in
+  // pieces of 4, 57 us in pieces of 2). Short items are not joined in a CTA for that.
+  const int fewest = s_longest > 8 ? static_cast<int>(sqrtf(static_cast<float>(s_longest))) : 1;
+  const int per = max(fewest, (total + static_cast<int>(gridDim.x) - 1) / static_cast<int>(gridDim.x));
   const int w0 = blockIdx.x * per;
   const int w_end = min(total, w0 + per);
   if (w0 >= w_end) return;  // the whole CTA; nothing is allocated yet
@@ -379,34 +386,31 @@ __global__ void __launch_bounds__(kThreads, 1)
     // A wait that gave up is recorded and stops the loader and the MMA warp; the rows go on to the
     // end over whatever TMEM holds (every later wait returns at once), so that barriers match.
     // This warp's 32 rows of a segment's Q into shared memory, D / 8 lanes to a row, whose place in
-    // memory comes from the lane that the row belongs to.
+    // memory comes from the lane that the row belongs to. Asynchronous copies, all in flight
+    // together; rows past the last are zeros.
     auto load_q = [&](const AttnCursor& q_at) {
-      constexpr int kLanes = D / 8, kRows = 32 / kLanes;  // per load
+      constexpr int kLanes = D / 8, kRows = 32 / kLanes;  // per copy
       const int fr = q_at.tile * kTile + st * kRowsPerStream + row;
       const int t = fr / p.group, head = q_at.head * p.group + fr - t * p.group;
-      const int64_t off = (q_at.req.q0 + t) * p.q_token_stride + head * p.q_head_stride;
-      const unsigned live_rows = __ballot_sync(0xffffffffu, fr < q_at.req.qlen * p.group);
-      const uint32_t flip = up.negate_q ? 0x80008000u : 0u;
-      const int ch = lane % kLanes;
-      unsigned char* dst = s_q + st * C::kTileBytes + (ch / 8) * C::kHalf;
-      uint4 v[32 / kRows];
+      const bool live = fr < q_at.req.qlen * p.group;
+      const int64_t off = live ? (q_at.req.q0 + t) * p.q_token_stride + head * p.q_head_stride : -1;
+      const int ch = lane % kLanes, first = (warp & 3) * 32 + lane / kLanes;
+      unsigned char* dst = s_q + st * C::kTileBytes + (ch / 8) * C::kHalf + first * 128;
+      const uint16_t* src = p.q + ch * 8;
 #pragma unroll
       for (int i = 0; i < 32 / kRows; ++i) {
-        const int from = i * kRows + lane / kLanes;
-        const int64_t src = __shfl_sync(0xffffffffu, off, from);
-        v[i] = make_uint4(0, 0, 0, 0);
-        if ((live_rows >> from) & 1u) {
-          v[i] = *reinterpret_cast<const uint4*>(p.q + src + ch * 8);
-          v[i].x ^= flip;
-          v[i].y ^= flip;
-          v[i].z ^= flip;
-          v[i].w ^= flip;
-        }
+        const int64_t from = __shfl_sync(0xffffffffu, off, i * kRows + lane / kLanes);
+        cp_async_16(dst + i * kRows * 128 + (((ch % 8) ^ ((first + i * kRows) & 7)) << 4),
+                    from >= 0 ? src + from : p.q, from >= 0 ? 16u : 0u);
       }
-#pragma unroll
-      for (int i = 0; i < 32 / kRows; ++i) {
-        const int q_row = (warp & 3) * 32 + i * kRows + lane / kLanes;
-        *reinterpret_cast<uint4*>(dst + q_row * 128 + (((ch % 8) ^ (q_row & 7)) << 4)) = v[i];
+      cp_async_wait_all();
+      if (up.negate_q) {  // each lane over what it copied
+#pragma unroll 1
+        for (int i = 0; i < 32 / kRows; ++i) {
+          uint4* v = reinterpret_cast<uint4*>(dst + i * kRows * 128 +
+                                              (((ch % 8) ^ ((first + i * kRows) & 7)) << 4));
+          *v = make_uint4(v->x ^ 0x80008000u, v->y ^ 0x80008000u, v->z ^ 0x80008000u, v->w ^ 0x80008000u);
+        }
       }
       fence_async_shared();
       mbar_arrive(&c.q_ready[st]);
