@@ -12,9 +12,9 @@
 // The weights are rounded to bf16 as the MMA's operand (the error of an output then has sqrt(2) times
 // the rms of its own rounding); their sum takes them unrounded.
 //
-// Measured: a 4096-token chunk over 16384 keys, 32 / 4 heads of 128: 750 us in short graph replays
-// (1280 TFLOP/s, 75 % of the burst GEMM rate), 876 us in stretches of seconds under the power cap
-// (1098 TFLOP/s, 77 % of the sustained rate). A block pair takes some 3500 cycles: 2300 from S to P
+// Measured: a 4096-token chunk over 16384 keys, 32 / 4 heads of 128: 731 us in short graph replays
+// (1316 TFLOP/s, 77 % of the burst GEMM rate), 854 us in stretches of seconds under the power cap
+// (1127 TFLOP/s, 79 % of the sustained rate). A block pair takes some 3500 cycles: 2300 from S to P
 // (read 160, maximum 400, exponentials 2 x 740) and 1200 from P to the next S, against 2048 of MMAs.
 // Tried without gain: part of the exponentials on the FMA pipe (782 - 852 us for 1/8 to 1/2 of them),
 // the first exponentials beside the maximum (884 us), MMAs issued from a lane-0 branch (1011 us: 84 to
