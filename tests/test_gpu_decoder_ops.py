@@ -666,3 +666,27 @@ def test_attention_negative_scale(cuda, D):
                                 scale=0.15 * sign, lse=lse)
             outs.append((out, lse))
         assert torch.equal(outs[0][0], outs[1][0]) and torch.equal(outs[0][1], outs[1][1])
+
+
+def test_attention_k_and_v_of_different_layouts(cuda):
+    """K with tokens before heads and V with heads before tokens, one kv head, one page, strides of one-sized
+    dimensions that mean nothing."""
+    g = _gen(cuda, 21)
+    ws = ops.attention_workspace(cuda)
+    for pages, Hkv in ((9, 2), (9, 1), (1, 2), (1, 1)):
+        kc = _bf16(g, pages, 16, Hkv, 64)
+        vc = _bf16(g, pages, Hkv, 16, 64).transpose(1, 2)
+        if Hkv == 1:
+            kc = kc.as_strided(kc.shape, (kc.stride(0), kc.stride(1), 0, 1))
+        if pages == 1:
+            vc = vc.as_strided(vc.shape, (0, *vc.stride()[1:]))
+        L = pages * 16 - 3
+        tables = torch.randperm(pages, device=cuda, generator=g).to(torch.int32)[None]
+        for n in (1, min(L, 50)):
+            q = _bf16(g, n, 4 * Hkv, 64)
+            out = torch.empty_like(q)
+            ops.paged_attention(q, kc, vc, tables, torch.tensor([L], dtype=torch.int32, device=cuda),
+                                torch.tensor([0, n], dtype=torch.int32, device=cuda), out, max_q_len=n,
+                                workspace=ws)
+            want, _, tol, _ = _attention64(q, kc, vc, tables, [L], [0, n], 64 ** -0.5, 0)
+            _within(out, want, tol)

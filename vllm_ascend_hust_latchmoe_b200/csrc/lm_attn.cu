@@ -11,6 +11,7 @@
 // keys and keeps its own running results; they are merged in shared memory (over the stage that
 // they read last) at the end of a segment. Segments of an item that several CTAs share are merged
 // through the workspace, by the CTA that arrives last, in the order of the keys.
+#include <algorithm>
 #include <string>
 
 #include "lm_attn.cuh"
@@ -354,16 +355,11 @@ __global__ void __launch_bounds__(kThreads, 1)
         if ((threadIdx.x & 15) == 0)
           *reinterpret_cast<float2*>(p.partial_ml + (slot * kTileRows + r) * 2) = make_float2(m, l);
       }
-      __threadfence();
       consumer_sync();
-      if (threadIdx.x == 0) {
-        c.last = atomicAdd(p.counters + cs, 1) == ce - cs;
-        if (c.last) p.counters[cs] = 0;  // every other CTA of the item has arrived
-      }
+      if (threadIdx.x == 0) c.last = attn_arrive(p.counters + cs, ce - cs + 1);
       consumer_sync();
       final = c.last != 0;
       if (final && live) {
-        __threadfence();
         // the common maximum first (a row's 16 threads share the partials), so that the sums'
         // loads do not wait for one another
         auto slot_of = [&](int k) { return (2 * static_cast<int64_t>(k) + (k == cs ? 1 : 0)) * kTileRows + r; };
@@ -451,6 +447,9 @@ int cache_map(CUtensorMap* out, const void* base, const AttnParams& a, int head_
               int64_t token_stride, int64_t head_stride, int box_rows, bool heads_first) {
   auto fn = tensor_map_encode_fn();
   if (fn == nullptr) return fail(LM_ERR_CUDA, "cuTensorMapEncodeTiled is unavailable");
+  // a dimension of one has no stride of its own
+  if (a.kv_heads == 1) head_stride = head_dim;
+  if (a.num_pages == 1) page_stride = std::max(token_stride, head_stride);
   const int h = heads_first ? 1 : 2, t = 3 - h;
   cuuint64_t dims[4], strides[3];
   cuuint32_t box[4] = {64, 1, 1, 1};

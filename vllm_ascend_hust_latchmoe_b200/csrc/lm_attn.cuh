@@ -250,6 +250,18 @@ __device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t parity, int32_
   return __all_sync(0xffffffffu, mbar_wait_bounded(bar, parity, err, abort_flag));
 }
 
+// One thread says that its CTA (or stream) has stored its partial result, and whether it was the last
+// of `pieces` to do so; the last one resets the counter. Between two barriers of the threads that
+// store and merge: this thread's fences order their stores before the count, and the others' partial
+// results before the merge.
+__device__ __forceinline__ bool attn_arrive(int32_t* counter, int pieces) {
+  __threadfence();
+  const bool last = atomicAdd(counter, 1) == pieces - 1;
+  if (last) *counter = 0;  // every other CTA of the item has arrived
+  __threadfence();
+  return last;
+}
+
 // The cache as TMA sees it: K and V by boxes of box_rows tokens (a divisor of the page size, at
 // most a block) of one head x 64 values, 128-byte swizzled.
 constexpr int kAttnBlock = 128;  // keys per block

@@ -34,6 +34,7 @@ constexpr int kRowsPerStream = 128;
 constexpr int kTile = 2 * kRowsPerStream;
 constexpr int kBlk = kAttnBlock;
 constexpr int kThreads = 384;
+constexpr int kSoftmaxRegs = 216, kOtherRegs = 72;  // per thread: 256 x 216 + 128 x 72 = 384 x 168
 constexpr float kRescaleAbove = 24.f;  // log2
 
 template <int D>
@@ -245,9 +246,9 @@ __global__ void __launch_bounds__(kThreads, 1)
   const uint32_t tmem = uniform(c.tmem_base);
   volatile int* abort_flag = &c.abort_flag;
 
-  // 256 softmax threads of 216 registers and 128 others of 72: the 384 x 168 of the launch
+  // the softmax threads' registers come from the other warps
   if (warp >= 8) {
-  asm volatile("setmaxnreg.dec.sync.aligned.u32 72;");
+  asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kOtherRegs));
   if (warp == 9 || warp == 11) {
     // ---------------------------------------------------------------------- K and V loaders
     attn_load_kv<D, kTile, C::kStages>(up, warp == 11, at, w0, w_end, s_kv, C::kTileBytes, warp == 11 ? 1 : 0, 2,
@@ -377,7 +378,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     }
   }
   } else {
-    asm volatile("setmaxnreg.inc.sync.aligned.u32 216;");
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kSoftmaxRegs));
     // ---------------------------------------------------------------------- softmax: a row per thread
     const int st = warp >> 2, row = threadIdx.x & 127;
     const uint32_t t_s = tmem + st * 256 + (static_cast<uint32_t>((warp & 3) * 32) << 16);
@@ -570,18 +571,12 @@ __global__ void __launch_bounds__(kThreads, 1)
             po[i * kTile] = make_float4(o[4 * i], o[4 * i + 1], o[4 * i + 2], o[4 * i + 3]);
         }
         *ml_of(me) = make_float2(m, l);  // a sum of 0: nothing seen, and perhaps no accumulator written
-        __threadfence();
         stream_sync(st);
-        if (row == 0) {
-          int32_t* counter = p.counters + 2 * cs + st;
-          c.last[st] = atomicAdd(counter, 1) == ce - cs;
-          if (c.last[st]) *counter = 0;  // every other CTA of the item has arrived
-        }
+        if (row == 0) c.last[st] = attn_arrive(p.counters + 2 * cs + st, ce - cs + 1);
         stream_sync(st);
         final = c.last[st] != 0;
         if (final && live) {
           // partials of CTAs cs .. ce, in the order of the keys whoever arrives last
-          __threadfence();
           m = -INFINITY;
 #pragma unroll 4
           for (int k = cs; k <= ce; ++k) {
@@ -641,10 +636,16 @@ int launch(const AttnLaunch& p, int ctas, cudaStream_t s) {
   cudaGetDevice(&dev);
   if (dev < 0 || dev >= 64) return fail(LM_ERR_UNSUPPORTED, "lm_paged_attention: device index >= 64");
   if (!done[dev]) {
-    const int rc = check_cuda(cudaFuncSetAttribute(paged_attn_umma_kernel<D>,
-                                                   cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                                   UmmaCfg<D>::kSmem),
-                              "lm_paged_attention: smem attribute");
+    // setmaxnreg hands out the registers that the CTA was launched with, and waits for ones that it
+    // does not have
+    cudaFuncAttributes attr;
+    int rc = check_cuda(cudaFuncGetAttributes(&attr, paged_attn_umma_kernel<D>), "lm_paged_attention: attributes");
+    if (!rc && attr.numRegs * kThreads < kSoftmaxRegs * 256 + kOtherRegs * 128)
+      rc = fail(LM_ERR_UNSUPPORTED, "lm_paged_attention: built with too few registers for its register split");
+    if (!rc)
+      rc = check_cuda(cudaFuncSetAttribute(paged_attn_umma_kernel<D>,
+                                           cudaFuncAttributeMaxDynamicSharedMemorySize, UmmaCfg<D>::kSmem),
+                      "lm_paged_attention: smem attribute");
     if (rc) return rc;
     done[dev] = true;
   }
