@@ -93,6 +93,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   extern __shared__ unsigned char smem_raw[];
   __shared__ int32_t s_warp[kThreads / 32];
   __shared__ RowsCtrl c;
+  __shared__ int s_longest;
   unsigned char* smem = reinterpret_cast<unsigned char*>(
       (reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~static_cast<uintptr_t>(1023));
   unsigned char* s_q = smem + S::kRing;
@@ -108,8 +109,10 @@ __global__ void __launch_bounds__(kThreads, 1)
       mbar_init(&c.q_empty[i], kWarps);
     }
     c.abort_flag = 0;
+    s_longest = 0;
     fence_mbarrier_init();
   }
+  __syncthreads();  // the barriers and s_longest are set
   if (warp == kWarps && lane == 0) {
     tma_prefetch_desc(&up.maps.k);
     tma_prefetch_desc(&up.maps.v);
@@ -120,16 +123,12 @@ __global__ void __launch_bounds__(kThreads, 1)
   // kernel has waited for both.
   if (!up.beside) pdl_wait();
   pdl_trigger();
-  attn_prefix<kTileRows, kBlock, kThreads>(p, s_prefix, s_warp);  // its barrier covers the inits too
-  const int total = s_prefix[p.num_requests];
-  const int per = (total + gridDim.x - 1) / gridDim.x;
-  int w = blockIdx.x * per;
-  const int w_end = min(total, w + per);
-  if (w >= w_end) {  // the whole CTA
-    pdl_wait();
+  int per, w, w_end;
+  AttnCursor at;
+  if (!attn_locate<kTileRows, kBlock, kThreads, false>(p, s_prefix, s_warp, &s_longest, per, w, w_end, at)) {
+    pdl_wait();  // the whole CTA
     return;
   }
-  AttnCursor at = attn_seek<kTileRows, kBlock>(p, s_prefix, w);
   volatile int* abort_flag = &c.abort_flag;
 
   if (warp < kWarps + 2 && warp >= kWarps) {

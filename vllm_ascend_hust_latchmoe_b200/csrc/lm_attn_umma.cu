@@ -216,6 +216,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     s_longest = 0;
     fence_mbarrier_init();
   }
+  __syncthreads();  // the barriers and s_longest are set
   if (warp == 9 && lane == 0) {
     tma_prefetch_desc(&up.maps.k);
     tma_prefetch_desc(&up.maps.v);
@@ -224,18 +225,13 @@ __global__ void __launch_bounds__(kThreads, 1)
   pdl_trigger();
   // the prefix lies where Q goes later
   int32_t* s_prefix = reinterpret_cast<int32_t*>(s_q);
-  __syncthreads();  // s_longest
-  attn_prefix<kTile, kBlk, kThreads>(p, s_prefix, s_warp, &s_longest);
-  const int total = s_prefix[p.num_requests];
   // A few long items are not cut into more pieces than pay: a block takes 1.9 us, another piece to
   // merge about as much, so n blocks are best cut into sqrt(n) pieces (16 items of 17 blocks: 42 us in
   // pieces of 4, 57 us in pieces of 2). Short items are not joined in a CTA for that.
-  const int fewest = s_longest > 8 ? static_cast<int>(sqrtf(static_cast<float>(s_longest))) : 1;
-  const int per = max(fewest, (total + static_cast<int>(gridDim.x) - 1) / static_cast<int>(gridDim.x));
-  const int w0 = blockIdx.x * per;
-  const int w_end = min(total, w0 + per);
-  if (w0 >= w_end) return;  // the whole CTA; nothing is allocated yet
-  AttnCursor at = attn_seek<kTile, kBlk>(p, s_prefix, w0);
+  int per, w0, w_end;
+  AttnCursor at;
+  if (!attn_locate<kTile, kBlk, kThreads, true>(p, s_prefix, s_warp, &s_longest, per, w0, w_end, at))
+    return;  // the whole CTA; nothing is allocated yet
   if (warp == 8) {
     tmem_alloc(&c.tmem_base, 512);
     tmem_relinquish();
@@ -248,135 +244,135 @@ __global__ void __launch_bounds__(kThreads, 1)
 
   // the softmax threads' registers come from the other warps
   if (warp >= 8) {
-  asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kOtherRegs));
-  if (warp == 9 || warp == 11) {
-    // ---------------------------------------------------------------------- K and V loaders
-    attn_load_kv<D, kTile, C::kStages>(up, warp == 11, at, w0, w_end, s_kv, C::kTileBytes, warp == 11 ? 1 : 0, 2,
-                                       c.kv_full, c.kv_empty, abort_flag);
-  } else if (warp == 8 || warp == 10) {
-    // ---------------------------------------------------------------------- MMA issuers, one a stream
-    const int st = warp == 8 ? 0 : 1;
-    const uint32_t idesc_s = idesc_bf16_f32(kRowsPerStream, kBlk);
-    const uint32_t idesc_o = idesc_bf16_f32(kRowsPerStream, D) | (1u << 16);  // B is N-major
-    const uint32_t kv_addr = uniform(smem_u32(s_kv));
-    const uint64_t q_desc = sdesc_k_sw128(uniform(smem_u32(s_q)) + st * C::kTileBytes);
-    const uint32_t t_s = tmem + st * 256, t_o = t_s + 128;
-    uint32_t q_phase = 0, p_phase = 0, kv_phase = 0;
-    uint32_t turn_phase = st == 0 ? 1u : 0u;  // stream 0 begins
-    int stage = 0;  // of the next tile, in the loader's order: K, V, K, V, ...
-    bool ok = true;
-    auto next_stage = [&]() {
-      if (++stage == C::kStages) {
-        stage = 0;
-        kv_phase ^= 1u;
-      }
-    };
-    auto release = [&](int tile, bool used) {  // after this stream's MMAs, if it had any
-      if (elect_one()) {
-        if (used)
-          umma_commit(&c.kv_empty[tile]);
-        else
-          mbar_arrive(&c.kv_empty[tile]);
-      }
-      __syncwarp();
-    };
-    auto issue_s = [&](int tile) {
-      const uint64_t k_desc = sdesc_k_sw128(uniform(kv_addr + tile * C::kTileBytes));
-      tc_fence_after();
-      if (elect_one()) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kOtherRegs));
+    if (warp == 9 || warp == 11) {
+      // ---------------------------------------------------------------------- K and V loaders
+      attn_load_kv<D, kTile, C::kStages>(up, warp == 11, at, w0, w_end, s_kv, C::kTileBytes, warp == 11 ? 1 : 0, 2,
+                                         c.kv_full, c.kv_empty, abort_flag);
+    } else {
+      // ---------------------------------------------------------------------- MMA issuers, one a stream
+      const int st = warp == 8 ? 0 : 1;
+      const uint32_t idesc_s = idesc_bf16_f32(kRowsPerStream, kBlk);
+      const uint32_t idesc_o = idesc_bf16_f32(kRowsPerStream, D) | (1u << 16);  // B is N-major
+      const uint32_t kv_addr = uniform(smem_u32(s_kv));
+      const uint64_t q_desc = sdesc_k_sw128(uniform(smem_u32(s_q)) + st * C::kTileBytes);
+      const uint32_t t_s = tmem + st * 256, t_o = t_s + 128;
+      uint32_t q_phase = 0, p_phase = 0, kv_phase = 0;
+      uint32_t turn_phase = st == 0 ? 1u : 0u;  // stream 0 begins
+      int stage = 0;  // of the next tile, in the loader's order: K, V, K, V, ...
+      bool ok = true;
+      auto next_stage = [&]() {
+        if (++stage == C::kStages) {
+          stage = 0;
+          kv_phase ^= 1u;
+        }
+      };
+      auto release = [&](int tile, bool used) {  // after this stream's MMAs, if it had any
+        if (elect_one()) {
+          if (used)
+            umma_commit(&c.kv_empty[tile]);
+          else
+            mbar_arrive(&c.kv_empty[tile]);
+        }
+        __syncwarp();
+      };
+      auto issue_s = [&](int tile) {
+        const uint64_t k_desc = sdesc_k_sw128(uniform(kv_addr + tile * C::kTileBytes));
+        tc_fence_after();
+        if (elect_one()) {
 #pragma unroll
-        for (int k = 0; k < D / 16; ++k) {
-          const uint64_t off = ((k / 4) * C::kHalf + (k % 4) * 32) >> 4;
-          umma_bf16(t_s, q_desc + off, k_desc + off, idesc_s, k > 0 ? 1u : 0u);
-        }
-        umma_commit(&c.s_full[st]);
-      }
-      __syncwarp();
-    };
-    for (int w = w0; w < w_end && ok;) {
-      const AttnSegment s = attn_segment<kTile, kBlk>(p, at, w, w_end);
-      const StreamRange r = stream_range(p, at, s, st);
-      if (r.end > r.begin) {
-        ok = warp_wait(&c.q_ready[st], q_phase, p.err, abort_flag);
-        q_phase ^= 1u;
-      }
-      if (s.blk0 < s.blk1 && ok) {  // S of the first block
-        ok = warp_wait(&c.kv_full[stage], kv_phase, p.err, abort_flag);
-        if (!ok) break;
-        const bool mine = s.blk0 == r.begin && r.end > r.begin;
-        if (mine) issue_s(stage);
-        release(stage, mine);
-        next_stage();
-      }
-      for (int blk = s.blk0; blk < s.blk1; ++blk) {  // P V of blk, S of blk + 1
-        const bool mine = blk >= r.begin && blk < r.end;
-        const int v_tile = stage;
-        const uint32_t v_phase = kv_phase;
-        next_stage();
-        if (blk + 1 < s.blk1) {
-          ok = warp_wait(&c.kv_full[stage], kv_phase, p.err, abort_flag);  // K arrives after V
-          if (!ok) break;
-        }
-        const bool next = blk + 1 >= r.begin && blk + 1 < r.end;
-        if constexpr (C::kOwnP) {  // S of the next block as soon as this one's has been read
-          if (mine) ok = warp_wait(&c.s_read[st], p_phase, p.err, abort_flag);
-          if (!ok) break;
-          if (next) issue_s(stage);
-          if (blk + 1 < s.blk1) release(stage, next);
-        }
-        ok = warp_wait(&c.kv_full[v_tile], v_phase, p.err, abort_flag);
-        if (!ok) break;
-        // The streams take turns, so that one's softmax runs beside the other's MMAs; left alone they
-        // fall into step, and exponentials and MMAs wait for their own kind (4096-token chunk over
-        // 16384 keys: 1027 against 909 us when it was tried, and 681 against 588 us with D = 64).
-        ok = warp_wait(&c.turn[st], turn_phase, p.err, abort_flag);
-        if (!ok) break;
-        turn_phase ^= 1u;
-        if (mine) {
-          // V rows of keys outside the tile's range, in a page that is partly inside (both streams
-          // write the same zeros)
-          const int r_lo = max(0, s.lo - blk * kBlk), r_hi = min(kBlk, s.hi - blk * kBlk);
-          if (r_lo > 0 || r_hi < kBlk) {
-            const uint4 zero = make_uint4(0, 0, 0, 0);
-            for (int i = lane; i < (kBlk - (r_hi - r_lo)) * (D / 8); i += 32) {
-              const int n = i / (D / 8), ch = i % (D / 8);
-              const int row = n < r_lo ? n : n - r_lo + r_hi;
-              *reinterpret_cast<uint4*>(s_kv + v_tile * C::kTileBytes + (ch / 8) * C::kHalf + row * 128 +
-                                        (ch % 8) * 16) = zero;
-            }
-            fence_async_shared();
-            __syncwarp();
+          for (int k = 0; k < D / 16; ++k) {
+            const uint64_t off = ((k / 4) * C::kHalf + (k % 4) * 32) >> 4;
+            umma_bf16(t_s, q_desc + off, k_desc + off, idesc_s, k > 0 ? 1u : 0u);
           }
-          const uint64_t v_desc = sdesc_mn_sw128(uniform(kv_addr + v_tile * C::kTileBytes), C::kHalf);
-          const uint32_t accumulate = uniform(blk > r.begin ? 1u : 0u);
-#pragma unroll
-          for (int part = 0; part < 2; ++part) {
-            ok = ok && warp_wait(part ? &c.p_ready[st] : &c.p_half[st], p_phase, p.err, abort_flag);
-            if (!ok) break;
-            tc_fence_after();
-            if (elect_one()) {
-#pragma unroll
-              for (int k = part * kBlk / 32; k < (part + 1) * kBlk / 32; ++k)
-                umma_bf16_ts(t_o, t_s + C::kColP + k * 8, v_desc + k * (2048 >> 4), idesc_o, k > 0 ? 1u : accumulate);
-              if (part == 1 && (C::kOwnP || blk == r.end - 1)) umma_commit(&c.o_full[st]);
-            }
-            __syncwarp();
-          }
-          if (!ok) break;
-          p_phase ^= 1u;
+          umma_commit(&c.s_full[st]);
         }
-        if (!C::kOwnP && next) issue_s(stage);
-        if (elect_one()) mbar_arrive(&c.turn[1 - st]);
-        release(v_tile, mine);
-        if (blk + 1 < s.blk1) {
-          if (!C::kOwnP) release(stage, next);
+        __syncwarp();
+      };
+      for (int w = w0; w < w_end && ok;) {
+        const AttnSegment s = attn_segment<kTile, kBlk>(p, at, w, w_end);
+        const StreamRange r = stream_range(p, at, s, st);
+        if (r.end > r.begin) {
+          ok = warp_wait(&c.q_ready[st], q_phase, p.err, abort_flag);
+          q_phase ^= 1u;
+        }
+        if (s.blk0 < s.blk1 && ok) {  // S of the first block
+          ok = warp_wait(&c.kv_full[stage], kv_phase, p.err, abort_flag);
+          if (!ok) break;
+          const bool mine = s.blk0 == r.begin && r.end > r.begin;
+          if (mine) issue_s(stage);
+          release(stage, mine);
           next_stage();
         }
+        for (int blk = s.blk0; blk < s.blk1; ++blk) {  // P V of blk, S of blk + 1
+          const bool mine = blk >= r.begin && blk < r.end;
+          const int v_tile = stage;
+          const uint32_t v_phase = kv_phase;
+          next_stage();
+          if (blk + 1 < s.blk1) {
+            ok = warp_wait(&c.kv_full[stage], kv_phase, p.err, abort_flag);  // K arrives after V
+            if (!ok) break;
+          }
+          const bool next = blk + 1 >= r.begin && blk + 1 < r.end;
+          if constexpr (C::kOwnP) {  // S of the next block as soon as this one's has been read
+            if (mine) ok = warp_wait(&c.s_read[st], p_phase, p.err, abort_flag);
+            if (!ok) break;
+            if (next) issue_s(stage);
+            if (blk + 1 < s.blk1) release(stage, next);
+          }
+          ok = warp_wait(&c.kv_full[v_tile], v_phase, p.err, abort_flag);
+          if (!ok) break;
+          // The streams take turns, so that one's softmax runs beside the other's MMAs; left alone they
+          // fall into step, and exponentials and MMAs wait for their own kind (4096-token chunk over
+          // 16384 keys: 1027 against 909 us when it was tried, and 681 against 588 us with D = 64).
+          ok = warp_wait(&c.turn[st], turn_phase, p.err, abort_flag);
+          if (!ok) break;
+          turn_phase ^= 1u;
+          if (mine) {
+            // V rows of keys outside the tile's range, in a page that is partly inside (both streams
+            // write the same zeros)
+            const int r_lo = max(0, s.lo - blk * kBlk), r_hi = min(kBlk, s.hi - blk * kBlk);
+            if (r_lo > 0 || r_hi < kBlk) {
+              const uint4 zero = make_uint4(0, 0, 0, 0);
+              for (int i = lane; i < (kBlk - (r_hi - r_lo)) * (D / 8); i += 32) {
+                const int n = i / (D / 8), ch = i % (D / 8);
+                const int row = n < r_lo ? n : n - r_lo + r_hi;
+                *reinterpret_cast<uint4*>(s_kv + v_tile * C::kTileBytes + (ch / 8) * C::kHalf + row * 128 +
+                                          (ch % 8) * 16) = zero;
+              }
+              fence_async_shared();
+              __syncwarp();
+            }
+            const uint64_t v_desc = sdesc_mn_sw128(uniform(kv_addr + v_tile * C::kTileBytes), C::kHalf);
+            const uint32_t accumulate = uniform(blk > r.begin ? 1u : 0u);
+#pragma unroll
+            for (int part = 0; part < 2; ++part) {
+              ok = ok && warp_wait(part ? &c.p_ready[st] : &c.p_half[st], p_phase, p.err, abort_flag);
+              if (!ok) break;
+              tc_fence_after();
+              if (elect_one()) {
+#pragma unroll
+                for (int k = part * kBlk / 32; k < (part + 1) * kBlk / 32; ++k)
+                  umma_bf16_ts(t_o, t_s + C::kColP + k * 8, v_desc + k * (2048 >> 4), idesc_o, k > 0 ? 1u : accumulate);
+                if (part == 1 && (C::kOwnP || blk == r.end - 1)) umma_commit(&c.o_full[st]);
+              }
+              __syncwarp();
+            }
+            if (!ok) break;
+            p_phase ^= 1u;
+          }
+          if (!C::kOwnP && next) issue_s(stage);
+          if (elect_one()) mbar_arrive(&c.turn[1 - st]);
+          release(v_tile, mine);
+          if (blk + 1 < s.blk1) {
+            if (!C::kOwnP) release(stage, next);
+            next_stage();
+          }
+        }
+        w += s.units;
+        if (w < w_end) attn_advance<kTile>(p, at);
       }
-      w += s.units;
-      if (w < w_end) attn_advance<kTile>(p, at);
     }
-  }
   } else {
     asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kSoftmaxRegs));
     // ---------------------------------------------------------------------- softmax: a row per thread
