@@ -690,3 +690,15 @@ def test_attention_k_and_v_of_different_layouts(cuda):
                                 workspace=ws)
             want, _, tol, _ = _attention64(q, kc, vc, tables, [L], [0, n], 64 ** -0.5, 0)
             _within(out, want, tol)
+
+
+@pytest.mark.parametrize("new", [1, 40])
+@pytest.mark.parametrize("B", [2, 13, 70, 149, 600])
+def test_attention_work_cut_anywhere(cuda, B, new):
+    """Lengths that let the CTAs' equal shares begin and end at every place of an item: ahead of its first block,
+    between its blocks, behind its last."""
+    rng = random.Random(B + new)
+    ws = ops.attention_workspace(cuda)
+    for top in (130, 700, 3000 if B < 100 else 1300):
+        _attention_case(cuda, [(rng.randint(0, top), rng.randint(1, new)) for _ in range(B)], 8, 1, 64, 16,
+                        workspace=ws, seed=top)

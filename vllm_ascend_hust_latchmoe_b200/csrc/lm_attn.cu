@@ -26,6 +26,11 @@ constexpr int kThreads = (kWarps + 3) * 32;  // and a loader each for K, V and Q
 constexpr int kTileRows = 16;
 constexpr int kSlice = 16;  // keys per warp and block
 constexpr int kBlock = kAttnBlock;
+// What an item costs beside its blocks, in blocks (its queries, its merge, a pipeline that runs dry):
+// 512 single tokens over 1 .. 1000 keys each, 40 query heads on 8, 282 us at 0, 220 at 1, 204 at 2,
+// 208 at 3; 64 over 1 .. 2000 keys, 32 heads on 4, 46, 37, 37 and 38 us. The price: few short
+// items spread over fewer CTAs (4 tokens over 1000 keys 10.8 -> 11.8 us).
+constexpr int kItem = 2;
 static_assert(kBlock == kWarps * kSlice, "a slice of every block per warp");
 
 __device__ __forceinline__ void ldmatrix_x4(uint32_t (&r)[4], uint32_t addr) {
@@ -125,7 +130,8 @@ __global__ void __launch_bounds__(kThreads, 1)
   pdl_trigger();
   int per, w, w_end;
   AttnCursor at;
-  if (!attn_locate<kTileRows, kBlock, kThreads, false>(p, s_prefix, s_warp, &s_longest, per, w, w_end, at)) {
+  if (!attn_locate<kTileRows, kBlock, kItem, kThreads, false>(p, s_prefix, s_warp, &s_longest, per, w, w_end,
+                                                              at)) {
     pdl_wait();  // the whole CTA
     return;
   }
@@ -133,15 +139,15 @@ __global__ void __launch_bounds__(kThreads, 1)
 
   if (warp < kWarps + 2 && warp >= kWarps) {
     const bool is_v = warp == kWarps + 1;
-    attn_load_kv<D, kTileRows, S::kStages>(up, is_v, at, w, w_end, smem + (is_v ? S::kTile : 0), S::kStage, 0, 1,
-                                           c.full, c.empty, abort_flag);
+    attn_load_kv<D, kTileRows, kItem, S::kStages>(up, is_v, at, w, w_end, smem + (is_v ? S::kTile : 0), S::kStage,
+                                                  0, 1, c.full, c.empty, abort_flag);
     pdl_wait();
     return;
   }
   if (warp > kWarps) {
     // ------------------------------------------------------------------------ queries
-    for (int seg = 0; w < w_end; ++seg) {
-      const AttnSegment s = attn_segment<kTileRows, kBlock>(p, at, w, w_end);
+    for (int seg = 0; attn_has<kItem>(at, w, w_end); ++seg) {
+      const AttnSegment s = attn_segment<kTileRows, kBlock, kItem>(p, at, w, w_end);
       if (s.blk1 > s.blk0) {
         if (!warp_wait(&c.q_empty[seg & 1], ((seg >> 1) & 1) ^ 1u, p.err, abort_flag)) break;
         const int rows = at.req.qlen * p.group;
@@ -157,7 +163,8 @@ __global__ void __launch_bounds__(kThreads, 1)
         cp_async_arrive_noinc(&c.q_full[seg & 1]);
       }
       w += s.units;
-      if (w < w_end) attn_advance<kTileRows>(p, at);
+      if (w >= w_end) break;
+      attn_advance<kTileRows>(p, at);
     }
     cp_async_wait_all();  // nothing in flight into shared memory when the warp leaves
     pdl_wait();
@@ -169,8 +176,8 @@ __global__ void __launch_bounds__(kThreads, 1)
   // whatever their stages hold (every later wait returns at once), so that their barriers match.
   const int g = lane >> 2, c2 = (lane & 3) * 2;
   int seq = 0;
-  for (int seg = 0; w < w_end; ++seg) {
-    const AttnSegment s = attn_segment<kTileRows, kBlock>(p, at, w, w_end);
+  for (int seg = 0; attn_has<kItem>(at, w, w_end); ++seg) {
+    const AttnSegment s = attn_segment<kTileRows, kBlock, kItem>(p, at, w, w_end);
     const int rows = at.req.qlen * p.group;
     const int row_base = at.tile * kTileRows;
     const int cached = at.req.seq - at.req.qlen;
@@ -343,7 +350,8 @@ __global__ void __launch_bounds__(kThreads, 1)
 
     bool final = s.whole;
     if (!s.whole) {
-      const int cs = s.start / per, ce = (s.end - 1) / per;
+      int cs, ce;
+      attn_holders<kItem>(s, per, cs, ce);
       const int me = blockIdx.x;
       const int64_t slot = 2 * static_cast<int64_t>(me) + (me == cs ? 1 : 0);
       if (live) {
@@ -408,7 +416,8 @@ __global__ void __launch_bounds__(kThreads, 1)
             l != 0.f ? (m + log2f(l)) * 0.693147180559945309f : -INFINITY;
     }
     w += s.units;
-    if (w < w_end) attn_advance<kTileRows>(p, at);
+    if (w >= w_end) break;
+    attn_advance<kTileRows>(p, at);
   }
   pdl_wait();
 }
@@ -541,11 +550,11 @@ extern "C" int lm_paged_attention(
     return fail(LM_ERR_INVALID_ARGUMENT, "lm_paged_attention: bad sizes (at most 4096 requests)");
   if (num_requests == 0 || num_tokens == 0) return LM_OK;
   if (num_pages == 0) return fail(LM_ERR_INVALID_ARGUMENT, "lm_paged_attention: an empty cache");
-  {  // the launches count their units (row tiles x key blocks) in 32 bits
+  {  // the launches count their units (row tiles x key blocks and 3 at most for each) in 32 bits
     const bool small = static_cast<int64_t>(max_q_len) * (num_q_heads / num_kv_heads) <= kTileRows;
     const int64_t tiles = num_tokens * num_q_heads / (small ? kTileRows : 2 * 128) +
                           static_cast<int64_t>(num_requests) * num_kv_heads;
-    const int64_t blocks = (static_cast<int64_t>(max_pages) * page_size + kBlock - 1) / kBlock + 1;
+    const int64_t blocks = (static_cast<int64_t>(max_pages) * page_size + kBlock - 1) / kBlock + 1 + 3;
     if (tiles > 0x7fffffff / blocks)
       return fail(LM_ERR_UNSUPPORTED, "lm_paged_attention: too much work for one call");
   }

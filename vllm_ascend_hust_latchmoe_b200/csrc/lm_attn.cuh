@@ -3,11 +3,13 @@
 //
 // Rows: a request's queries of one kv head are flattened to (token, query head of the group)
 // rows, so a row tile fills up whatever the number of query heads per kv head. An item is
-// (request, kv head, row tile); its cost is the number of kv blocks that its rows see. All items'
-// blocks are laid end to end and every CTA takes the same number of them, wherever that cuts an
-// item ("per" units each): the load is even whatever the requests' lengths, and one long sequence
-// spreads over the whole GPU. A CTA leaves at most two partial results: one of the item that it
-// continues and one of the item that it starts and does not finish.
+// (request, kv head, row tile); its cost is ITEM units, for what it takes whatever its length, and
+// one for each kv block that its rows see. All items' units are laid end to end and every CTA takes
+// the same number of them, wherever that cuts an item ("per" units each): the load is even whatever
+// the requests' lengths, and one long sequence spreads over the whole GPU. A boundary among an
+// item's ITEM first units leaves all of the item to the CTA behind it. A CTA leaves at most two
+// partial results: one of the item that it continues and one of the item that it starts and does
+// not finish.
 #pragma once
 
 #include <cuda.h>
@@ -91,9 +93,9 @@ __device__ __forceinline__ int attn_tiles(const AttnParams& p, const AttnRequest
   return rows >= p.min_rows && rows <= p.max_rows ? (rows + TILE_ROWS - 1) / TILE_ROWS : 0;
 }
 
-// Key blocks of a lane's request per kv head, and the longest of its items; the lanes of the warp
+// Units of a lane's request per kv head, and the most blocks of its items; the lanes of the warp
 // share the tiles of a request that has several. All lanes call it (tiles 0: no request).
-template <int TILE_ROWS, int BLOCK>
+template <int TILE_ROWS, int BLOCK, int ITEM>
 __device__ __forceinline__ int attn_cost(const AttnParams& p, const AttnRequest& r, int tiles, int& longest) {
   int cost = 0;
   if (tiles == 1) {
@@ -101,6 +103,7 @@ __device__ __forceinline__ int attn_cost(const AttnParams& p, const AttnRequest&
     attn_tile_keys<TILE_ROWS>(p, r, 0, lo, hi);
     cost = attn_blocks<BLOCK>(lo, hi);
     longest = max(longest, cost);
+    cost += ITEM;
   }
   for (unsigned many = __ballot_sync(0xffffffffu, tiles > 1); many != 0; many &= many - 1) {
     const int src = __ffs(many) - 1;
@@ -114,7 +117,7 @@ __device__ __forceinline__ int attn_cost(const AttnParams& p, const AttnRequest&
       int lo, hi;
       attn_tile_keys<TILE_ROWS>(p, o, t, lo, hi);
       const int n_blocks = attn_blocks<BLOCK>(lo, hi);
-      part += n_blocks;
+      part += n_blocks + ITEM;
       longest = max(longest, n_blocks);
     }
     part = __reduce_add_sync(0xffffffffu, part);
@@ -125,7 +128,7 @@ __device__ __forceinline__ int attn_cost(const AttnParams& p, const AttnRequest&
 
 // Exclusive prefix of the requests' costs in s_prefix[0 .. B], and the longest item's blocks (into
 // *s_longest, zeroed by the caller ahead of a barrier). Called by all NT threads, a request each.
-template <int TILE_ROWS, int BLOCK, int NT>
+template <int TILE_ROWS, int BLOCK, int ITEM, int NT>
 __device__ __forceinline__ void attn_prefix(const AttnParams& p, int32_t* s_prefix, int32_t* s_warp,
                                             int* s_longest) {
   const int B = p.num_requests;
@@ -140,7 +143,7 @@ __device__ __forceinline__ void attn_prefix(const AttnParams& p, int32_t* s_pref
       r = attn_request(p, b, blockIdx.x == 0);
       tiles = attn_tiles<TILE_ROWS>(p, r);
     }
-    const int cost = attn_cost<TILE_ROWS, BLOCK>(p, r, tiles, longest);
+    const int cost = attn_cost<TILE_ROWS, BLOCK, ITEM>(p, r, tiles, longest);
     if (b < b1) s_prefix[b + 1] = cost * p.kv_heads;
     sum += cost * p.kv_heads;
   }
@@ -170,9 +173,16 @@ struct AttnCursor {
   int b, head, tile, tiles, off;
 };
 
+// Whether some of the cursor's blocks lie before w_end (a boundary ahead of an item's first block
+// leaves the item to the next CTA).
+template <int ITEM>
+__device__ __forceinline__ bool attn_has(const AttnCursor& c, int w, int w_end) {
+  return w_end - w + c.off > ITEM;
+}
+
 // Sets the head and tile of a cursor whose `off` counts from its request's first unit; every warp
 // computes it alike.
-template <int TILE_ROWS, int BLOCK>
+template <int TILE_ROWS, int BLOCK, int ITEM>
 __device__ __forceinline__ void attn_enter(const AttnParams& p, AttnCursor& c, int request_units) {
   const int per_head = request_units / p.kv_heads;
   c.head = c.off / per_head;
@@ -183,7 +193,7 @@ __device__ __forceinline__ void attn_enter(const AttnParams& p, AttnCursor& c, i
     int lo, hi, n = 0;
     if (t < c.tiles) {
       attn_tile_keys<TILE_ROWS>(p, c.req, t, lo, hi);
-      n = attn_blocks<BLOCK>(lo, hi);
+      n = attn_blocks<BLOCK>(lo, hi) + ITEM;
     }
     int incl = n;
 #pragma unroll
@@ -207,7 +217,7 @@ __device__ __forceinline__ void attn_enter(const AttnParams& p, AttnCursor& c, i
 // it has none. FEW: items longer than 8 blocks are cut into sqrt(n) pieces at most. Up to 32 requests
 // every warp works it out for itself, a request a lane; more go through shared memory (0.2 to 0.7 us
 // more: 16 single tokens over 1000 keys 16.4 against 15.8 us).
-template <int TILE_ROWS, int BLOCK, int NT, bool FEW>
+template <int TILE_ROWS, int BLOCK, int ITEM, int NT, bool FEW>
 __device__ __forceinline__ bool attn_locate(const AttnParams& p, int32_t* s_prefix, int32_t* s_warp,
                                             int* s_longest, int& per, int& w, int& w_end, AttnCursor& c) {
   const int B = p.num_requests, lane = threadIdx.x & 31;
@@ -218,7 +228,7 @@ __device__ __forceinline__ bool attn_locate(const AttnParams& p, int32_t* s_pref
       r = attn_request(p, lane, blockIdx.x == 0 && threadIdx.x < 32);
       tiles = attn_tiles<TILE_ROWS>(p, r);
     }
-    units = attn_cost<TILE_ROWS, BLOCK>(p, r, tiles, longest) * p.kv_heads;
+    units = attn_cost<TILE_ROWS, BLOCK, ITEM>(p, r, tiles, longest) * p.kv_heads;
     longest = __reduce_max_sync(0xffffffffu, longest);
     incl = units;
 #pragma unroll
@@ -228,7 +238,7 @@ __device__ __forceinline__ bool attn_locate(const AttnParams& p, int32_t* s_pref
     }
     total = __shfl_sync(0xffffffffu, incl, 31);
   } else {
-    attn_prefix<TILE_ROWS, BLOCK, NT>(p, s_prefix, s_warp, s_longest);
+    attn_prefix<TILE_ROWS, BLOCK, ITEM, NT>(p, s_prefix, s_warp, s_longest);
     total = s_prefix[B];
     longest = *s_longest;
   }
@@ -257,8 +267,12 @@ __device__ __forceinline__ bool attn_locate(const AttnParams& p, int32_t* s_pref
     c.off = w - s_prefix[lo_b];
     units = s_prefix[lo_b + 1] - s_prefix[lo_b];
   }
-  attn_enter<TILE_ROWS, BLOCK>(p, c, units);
-  return true;
+  attn_enter<TILE_ROWS, BLOCK, ITEM>(p, c, units);
+  if (c.off <= ITEM) {  // the boundary falls ahead of the item's first block: it is this CTA's from there
+    w -= c.off;
+    c.off = 0;
+  }
+  return attn_has<ITEM>(c, w, w_end);
 }
 
 // To the next item; only called when there is one.
@@ -285,19 +299,27 @@ struct AttnSegment {
   bool whole;
 };
 
-template <int TILE_ROWS, int BLOCK>
+template <int TILE_ROWS, int BLOCK, int ITEM>
 __device__ __forceinline__ AttnSegment attn_segment(const AttnParams& p, const AttnCursor& c, int w,
                                                     int w_end) {
   AttnSegment s;
   attn_tile_keys<TILE_ROWS>(p, c.req, c.tile, s.lo, s.hi);
   const int n = attn_blocks<BLOCK>(s.lo, s.hi);
   s.start = w - c.off;
-  s.end = s.start + n;
-  s.units = min(n - c.off, w_end - w);
-  s.whole = c.off == 0 && s.units == n;
-  s.blk0 = s.lo / BLOCK + c.off;
-  s.blk1 = s.hi > s.lo ? s.blk0 + s.units : s.blk0;
+  s.end = s.start + ITEM + n;
+  s.units = min(s.end, w_end) - w;
+  const int b0 = max(c.off - ITEM, 0), b1 = c.off + s.units - ITEM;
+  s.whole = b0 == 0 && b1 == n;
+  s.blk0 = s.lo / BLOCK + b0;
+  s.blk1 = s.hi > s.lo ? s.lo / BLOCK + b1 : s.blk0;
   return s;
+}
+
+// The first and last CTA that hold blocks of a segment's item.
+template <int ITEM>
+__device__ __forceinline__ void attn_holders(const AttnSegment& s, int per, int& first, int& last) {
+  first = (s.start + ITEM) / per;
+  last = (s.end - 1) / per;
 }
 
 // A bounded wait of a whole warp, with one answer for all of its lanes.
@@ -356,7 +378,7 @@ __device__ __forceinline__ void fence_async_shared() {
 // segment's item come from boxes past the cache's end, which TMA fills with zeros; inside a box
 // that is partly in range, the cache's own contents arrive. One warp for both would not do: with
 // pages of 16 keys (boxes of 2 KB) a warp issues 34 GB/s.
-template <int D, int TILE_ROWS, int STAGES>
+template <int D, int TILE_ROWS, int ITEM, int STAGES>
 __device__ __forceinline__ void attn_load_kv(const AttnLaunch& up, bool is_v, AttnCursor at, int w,
                                              int w_end, unsigned char* ring, int stage_bytes, int first,
                                              int step, uint64_t* full, uint64_t* empty,
@@ -370,8 +392,8 @@ __device__ __forceinline__ void attn_load_kv(const AttnLaunch& up, bool is_v, At
   const CUtensorMap* map = is_v ? &up.maps.v : &up.maps.k;
   int stage = first % STAGES, passes = 0, tiles = 0;
   bool ok = true;
-  while (w < w_end && ok) {
-    const AttnSegment s = attn_segment<TILE_ROWS, kAttnBlock>(p, at, w, w_end);
+  while (attn_has<ITEM>(at, w, w_end) && ok) {
+    const AttnSegment s = attn_segment<TILE_ROWS, kAttnBlock, ITEM>(p, at, w, w_end);
     const int32_t* table = p.tables + at.b * p.table_stride;
     auto page_of = [&](int blk) {  // the page of this lane's box, num_pages where there is none
       const int tok = blk * kAttnBlock + box * up.maps.box_rows;
@@ -405,7 +427,8 @@ __device__ __forceinline__ void attn_load_kv(const AttnLaunch& up, bool is_v, At
       page = page_next;
     }
     w += s.units;
-    if (w < w_end) attn_advance<TILE_ROWS>(p, at);
+    if (w >= w_end) break;
+    attn_advance<TILE_ROWS>(p, at);
   }
   // Every stage used is released before the CTA may leave (no copy or commit is in flight then); of
   // two warps that fill the ring in turn, the one that ends last sees the last pass of each stage.

@@ -17,7 +17,9 @@
 // (1127 TFLOP/s, 79 % of the sustained rate). A block pair takes some 3500 cycles: 2300 from S to P
 // (read 160, maximum 400, exponentials 2 x 740) and 1200 from P to the next S, against 2048 of MMAs.
 // Tried without gain: part of the exponentials on the FMA pipe (782 - 852 us for 1/8 to 1/2 of them),
-// the first exponentials beside the maximum (884 us), MMAs issued from a lane-0 branch (1011 us: 84 to
+// the first exponentials beside the maximum (884 us), the next item's Q begun ahead of its
+// predecessor's last softmax (3 % slower), results exchanged between lanes for wider stores (a prompt
+// of 4096 tokens -3 %, eight of 1024 +5 %), MMAs issued from a lane-0 branch (1011 us: 84 to
 // 128 cycles an instruction against 70 with elect.sync and operands that the compiler sees uniform).
 //
 // A row's reference maximum moves (and O is rescaled) only when a block's maximum exceeds it by a
@@ -33,6 +35,11 @@ namespace {
 constexpr int kRowsPerStream = 128;
 constexpr int kTile = 2 * kRowsPerStream;
 constexpr int kBlk = kAttnBlock;
+// What an item costs beside its blocks, in blocks (its queries, masks and results; 7,000 to 9,000
+// cycles against 3,100 for a block): a prompt of 4096 tokens, 64 query heads on 4, 469 us at 0, 318
+// at 2, 277 at 3, 264 at 4, 272 at 6; 8 requests of 1 to 1000 new tokens over 3000 54.5, 51.6, 51.0,
+// 52.1 and 53.4 us.
+constexpr int kItem = 3;
 constexpr int kThreads = 384;
 constexpr int kSoftmaxRegs = 216, kOtherRegs = 72;  // per thread: 256 x 216 + 128 x 72 = 384 x 168
 constexpr float kRescaleAbove = 24.f;  // log2
@@ -230,7 +237,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   // pieces of 4, 57 us in pieces of 2). Short items are not joined in a CTA for that.
   int per, w0, w_end;
   AttnCursor at;
-  if (!attn_locate<kTile, kBlk, kThreads, true>(p, s_prefix, s_warp, &s_longest, per, w0, w_end, at))
+  if (!attn_locate<kTile, kBlk, kItem, kThreads, true>(p, s_prefix, s_warp, &s_longest, per, w0, w_end, at))
     return;  // the whole CTA; nothing is allocated yet
   if (warp == 8) {
     tmem_alloc(&c.tmem_base, 512);
@@ -247,8 +254,8 @@ __global__ void __launch_bounds__(kThreads, 1)
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kOtherRegs));
     if (warp == 9 || warp == 11) {
       // ---------------------------------------------------------------------- K and V loaders
-      attn_load_kv<D, kTile, C::kStages>(up, warp == 11, at, w0, w_end, s_kv, C::kTileBytes, warp == 11 ? 1 : 0, 2,
-                                         c.kv_full, c.kv_empty, abort_flag);
+      attn_load_kv<D, kTile, kItem, C::kStages>(up, warp == 11, at, w0, w_end, s_kv, C::kTileBytes,
+                                                warp == 11 ? 1 : 0, 2, c.kv_full, c.kv_empty, abort_flag);
     } else {
       // ---------------------------------------------------------------------- MMA issuers, one a stream
       const int st = warp == 8 ? 0 : 1;
@@ -289,8 +296,8 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
         __syncwarp();
       };
-      for (int w = w0; w < w_end && ok;) {
-        const AttnSegment s = attn_segment<kTile, kBlk>(p, at, w, w_end);
+      for (int w = w0; attn_has<kItem>(at, w, w_end) && ok;) {
+        const AttnSegment s = attn_segment<kTile, kBlk, kItem>(p, at, w, w_end);
         const StreamRange r = stream_range(p, at, s, st);
         if (r.end > r.begin) {
           ok = warp_wait(&c.q_ready[st], q_phase, p.err, abort_flag);
@@ -370,7 +377,8 @@ __global__ void __launch_bounds__(kThreads, 1)
           }
         }
         w += s.units;
-        if (w < w_end) attn_advance<kTile>(p, at);
+        if (w >= w_end) break;
+        attn_advance<kTile>(p, at);
       }
     }
   } else {
@@ -412,10 +420,11 @@ __global__ void __launch_bounds__(kThreads, 1)
       fence_async_shared();
       mbar_arrive(&c.q_ready[st]);
     };
-    AttnSegment s = attn_segment<kTile, kBlk>(p, at, w0, w_end);
+    AttnSegment s = attn_segment<kTile, kBlk, kItem>(p, at, w0, w_end);
     StreamRange r = stream_range(p, at, s, st);
     if (r.end > r.begin) load_q(at);
-    for (int w = w0; w < w_end;) {
+    bool more = true;
+    for (int w = w0; more;) {
       const int rows = at.req.qlen * p.group, cached = at.req.seq - at.req.qlen;
       const int fr = at.tile * kTile + st * kRowsPerStream + row;  // flattened row
       const bool live = fr < rows;
@@ -521,9 +530,13 @@ __global__ void __launch_bounds__(kThreads, 1)
       const AttnSegment ds = s;
       const StreamRange dr = r;
       w += s.units;
-      if (w < w_end) {
+      more = w < w_end;
+      if (more) {
         attn_advance<kTile>(p, at);
-        s = attn_segment<kTile, kBlk>(p, at, w, w_end);
+        more = attn_has<kItem>(at, w, w_end);
+      }
+      if (more) {
+        s = attn_segment<kTile, kBlk, kItem>(p, at, w, w_end);
         r = stream_range(p, at, s, st);
         if (r.end > r.begin) load_q(at);
       }
@@ -551,7 +564,9 @@ __global__ void __launch_bounds__(kThreads, 1)
       };
       if (has_o) read_o();
       if (!ds.whole) {
-        const int cs = ds.start / per, ce = (ds.end - 1) / per, me = blockIdx.x;
+        int cs, ce;
+        attn_holders<kItem>(ds, per, cs, ce);
+        const int me = blockIdx.x;
         // partial results lie as [D / 4][256 rows][4]: a warp's 16-byte pieces are neighbours
         auto slot_of = [&](int k) { return 2 * static_cast<int64_t>(k) + (k == cs ? 1 : 0); };
         auto o_of = [&](int k) {
