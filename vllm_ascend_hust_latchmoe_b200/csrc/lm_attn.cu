@@ -28,8 +28,8 @@ constexpr int kSlice = 16;  // keys per warp and block
 constexpr int kBlock = kAttnBlock;
 // What an item costs beside its blocks, in blocks (its queries, its merge, a pipeline that runs dry):
 // 512 single tokens over 1 .. 1000 keys each, 40 query heads on 8, 282 us at 0, 220 at 1, 204 at 2,
-// 208 at 3; 64 over 1 .. 2000 keys, 32 heads on 4, 46, 37, 37 and 38 us. The price: few short
-// items spread over fewer CTAs (4 tokens over 1000 keys 10.8 -> 11.8 us).
+// 208 at 3 (189 since items became cheaper); 64 over 1 .. 2000 keys, 32 heads on 4, 46, 37, 37 and
+// 38 us. The price: few short items spread over fewer CTAs (4 tokens over 1000 keys 10.8 -> 11.8 us).
 constexpr int kItem = 2;
 static_assert(kBlock == kWarps * kSlice, "a slice of every block per warp");
 
@@ -156,7 +156,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         for (int j = 0; j < kTileRows * kChunks / 32; ++j) {
           const int r = (j * 32 + lane) / kChunks, ch = (j * 32 + lane) % kChunks;
           const int row = at.tile * kTileRows + r;
-          const int t = row / p.group, head = at.head * p.group + row - t * p.group;
+          const int t = p.by_group(row), head = at.head * p.group + row - t * p.group;
           const uint16_t* src = p.q + (at.req.q0 + t) * p.q_token_stride + head * p.q_head_stride + ch * 8;
           cp_async_16(dst + q_at<D>(r, ch), row < rows ? src : p.q, row < rows ? 16u : 0u);
         }
@@ -198,7 +198,7 @@ __global__ void __launch_bounds__(kThreads, 1)
 
     // keys (j > low, j <= high) that rows g and g + 8 of the tile see
     const int r0 = row_base + g, r1 = r0 + 8;
-    const int t0 = r0 / p.group, t1 = r1 / p.group;
+    const int t0 = p.by_group(r0), t1 = p.by_group(r1);
     const int high0 = r0 < rows ? cached + t0 : -1;
     const int high1 = r1 < rows ? cached + t1 : -1;
     const int low0 = p.window > 0 ? cached + t0 - p.window : -1;
@@ -257,8 +257,8 @@ __global__ void __launch_bounds__(kThreads, 1)
       }
       if (__any_sync(0xffffffffu, mx0 > m0 || mx1 > m1)) {
         const float n0 = fmaxf(m0, mx0), n1 = fmaxf(m1, mx1);
-        const float f0 = m0 == -INFINITY ? 0.f : exp2f(m0 - n0);
-        const float f1 = m1 == -INFINITY ? 0.f : exp2f(m1 - n1);
+        const float f0 = m0 == -INFINITY ? 0.f : ex2(m0 - n0);
+        const float f1 = m1 == -INFINITY ? 0.f : ex2(m1 - n1);
         m0 = n0;
         m1 = n1;
         l0 *= f0;
@@ -275,8 +275,8 @@ __global__ void __launch_bounds__(kThreads, 1)
       uint32_t pa[4];
 #pragma unroll
       for (int n = 0; n < 2; ++n) {
-        const float e0 = exp2f(sc[n][0] - b0), e1 = exp2f(sc[n][1] - b0);
-        const float e2 = exp2f(sc[n][2] - b1), e3 = exp2f(sc[n][3] - b1);
+        const float e0 = ex2(sc[n][0] - b0), e1 = ex2(sc[n][1] - b0);
+        const float e2 = ex2(sc[n][2] - b1), e3 = ex2(sc[n][3] - b1);
         l0 += e0 + e1;
         l1 += e2 + e3;
         pa[2 * n] = pack_bf16x2(e0, e1);
@@ -332,7 +332,7 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll
       for (int k = 0; k < kWarps; ++k) {
         const float mk = c.ml[k][r][0];
-        const float f = mk == -INFINITY ? 0.f : exp2f(mk - m);
+        const float f = mk == -INFINITY ? 0.f : ex2(mk - m);
         l += f * c.ml[k][r][1];
         const float* src = results + (k * kTileRows + r) * D + (((col >> 3) ^ (r & 7)) * 8 + (col & 7));
 #pragma unroll
@@ -384,7 +384,7 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll 8
         for (int k = cs; k <= ce; ++k) {
           const float2 ml = ml_of(k);
-          const float f = ml.x == -INFINITY ? 0.f : exp2f(ml.x - m);
+          const float f = ml.x == -INFINITY ? 0.f : ex2(ml.x - m);
           const float* src = p.partial_o + slot_of(k) * D + col;
           l += f * ml.y;
 #pragma unroll
@@ -399,8 +399,9 @@ __global__ void __launch_bounds__(kThreads, 1)
       }
     }
     if (final && live) {
-      const int tok = at.req.q0 + (row_base + r) / p.group;
-      const int head = at.head * p.group + (row_base + r) % p.group;
+      const int t = p.by_group(row_base + r);
+      const int tok = at.req.q0 + t;
+      const int head = at.head * p.group + row_base + r - t * p.group;
       const float inv = l != 0.f ? 1.f / l : 0.f;
       uint16_t* dst = p.out + tok * p.out_token_stride + head * p.out_head_stride + col;
       uint32_t packed[kCols / 2];
@@ -599,7 +600,9 @@ extern "C" int lm_paged_attention(
   p.q_heads = num_q_heads;
   p.kv_heads = num_kv_heads;
   p.group = num_q_heads / num_kv_heads;
+  p.by_group = attn_div(p.group);
   p.page_size = page_size;
+  p.by_page = attn_div(page_size);
   p.num_pages = static_cast<int>(num_pages);
   p.max_pages = max_pages;
   p.window = window;

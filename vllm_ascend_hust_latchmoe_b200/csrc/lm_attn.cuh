@@ -22,6 +22,24 @@ constexpr int kAttnMaxRequests = 4096;
 constexpr int kAttnMaxCtas = 512;      // counters in the workspace
 constexpr int kAttnMaxPartialRows = 256;
 
+// n / d for 0 <= n < 2^31 as a product and a shift: mul = ceil(2^shift / d) with shift = 31 +
+// ceil(log2 d) is above 2^shift / d by less than 2^(shift - 31) / d, which n is too small to show.
+// (Divisions by numbers that come as arguments took 15 % of an item of one block.)
+struct AttnDiv {
+  uint32_t mul;
+  int shift;
+  __device__ __forceinline__ int operator()(int n) const {
+    return static_cast<int>((static_cast<uint64_t>(static_cast<uint32_t>(n)) * mul) >> shift);
+  }
+};
+
+inline AttnDiv attn_div(int d) {
+  AttnDiv r{0, 31};
+  while ((int64_t{1} << (r.shift - 31)) < d) ++r.shift;
+  r.mul = static_cast<uint32_t>(((uint64_t{1} << r.shift) + d - 1) / d);
+  return r;
+}
+
 struct AttnParams {
   const uint16_t* q;
   const uint16_t* k;
@@ -41,6 +59,7 @@ struct AttnParams {
   int64_t table_stride;
   int64_t num_tokens;
   int num_requests, q_heads, kv_heads, group, page_size, num_pages, max_pages, window;
+  AttnDiv by_group, by_page;
   int min_rows, max_rows;  // requests with this many rows per kv head are this launch's
   float scale_log2;        // softmax scale * log2(e)
 };
@@ -73,8 +92,8 @@ template <int TILE_ROWS>
 __device__ __forceinline__ void attn_tile_keys(const AttnParams& p, const AttnRequest& r, int tile,
                                                int& lo, int& hi) {
   const int rows = r.qlen * p.group;
-  const int first = tile * TILE_ROWS / p.group;
-  const int last = (min((tile + 1) * TILE_ROWS, rows) - 1) / p.group;
+  const int first = p.by_group(tile * TILE_ROWS);
+  const int last = p.by_group(min((tile + 1) * TILE_ROWS, rows) - 1);
   const int cached = r.seq - r.qlen;  // negative: the first queries stand before every key
   hi = max(0, cached + last + 1);
   lo = p.window > 0 ? min(hi, max(0, cached + first - p.window + 1)) : 0;
@@ -322,6 +341,14 @@ __device__ __forceinline__ void attn_holders(const AttnSegment& s, int per, int&
   last = (s.end - 1) / per;
 }
 
+// 2^x. Weights below 2^-126 of a row's largest are flushed: they are far below its rounding (exp2f, which
+// keeps them, cost 1 % of decode steps of few keys).
+__device__ __forceinline__ float ex2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
 // A bounded wait of a whole warp, with one answer for all of its lanes.
 __device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t parity, int32_t* err,
                                           volatile int* abort_flag) {
@@ -398,7 +425,7 @@ __device__ __forceinline__ void attn_load_kv(const AttnLaunch& up, bool is_v, At
     auto page_of = [&](int blk) {  // the page of this lane's box, num_pages where there is none
       const int tok = blk * kAttnBlock + box * up.maps.box_rows;
       if (lane >= n_loads || tok >= s.hi || tok + up.maps.box_rows <= s.lo) return p.num_pages;
-      const int pg = table[tok / p.page_size];
+      const int pg = table[p.by_page(tok)];
       if (pg < 0 || pg >= p.num_pages) {
         record_error(p.err, LM_DEVERR_BAD_PAGE);
         return p.num_pages;
@@ -408,7 +435,8 @@ __device__ __forceinline__ void attn_load_kv(const AttnLaunch& up, bool is_v, At
     int page = s.blk0 < s.blk1 ? page_of(s.blk0) : 0;
     for (int blk = s.blk0; blk < s.blk1 && ok; ++blk) {
       const int page_next = blk + 1 < s.blk1 ? page_of(blk + 1) : 0;
-      const int y = (blk * kAttnBlock + box * up.maps.box_rows) % p.page_size;
+      const int tok = blk * kAttnBlock + box * up.maps.box_rows;
+      const int y = tok - p.by_page(tok) * p.page_size;
       ok = warp_wait(&empty[stage], (passes & 1u) ^ 1u, p.err, abort_flag);
       if (!ok) break;
       if (lane == 0) mbar_arrive_expect_tx(&full[stage], kTileBytes);

@@ -12,9 +12,9 @@
 // The weights are rounded to bf16 as the MMA's operand (the error of an output then has sqrt(2) times
 // the rms of its own rounding); their sum takes them unrounded.
 //
-// Measured: a 4096-token chunk over 16384 keys, 32 / 4 heads of 128: 731 us in short graph replays
-// (1316 TFLOP/s, 77 % of the burst GEMM rate), 854 us in stretches of seconds under the power cap
-// (1127 TFLOP/s, 79 % of the sustained rate). A block pair takes some 3500 cycles: 2300 from S to P
+// Measured: a 4096-token chunk over 16384 keys, 32 / 4 heads of 128: 737 to 760 us in short graph
+// replays (1265 to 1305 TFLOP/s, 74 to 77 % of the burst GEMM rate), 862 us in stretches of seconds
+// under the power cap (1117 TFLOP/s, 78 % of the sustained rate). A block pair takes some 3500 cycles: 2300 from S to P
 // (read 160, maximum 400, exponentials 2 x 740) and 1200 from P to the next S, against 2048 of MMAs.
 // Tried without gain: part of the exponentials on the FMA pipe (782 - 852 us for 1/8 to 1/2 of them),
 // the first exponentials beside the maximum (884 us), the next item's Q begun ahead of its
@@ -125,12 +125,6 @@ __device__ __forceinline__ void tmem_st_32x32b_x32(uint32_t taddr, const uint32_
 
 __device__ __forceinline__ void tmem_st_wait() {
   asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
-}
-
-__device__ __forceinline__ float ex2(float x) {
-  float y;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-  return y;
 }
 
 // Two floats in one register pair: the FMA pipe does both in one instruction.
@@ -396,7 +390,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     auto load_q = [&](const AttnCursor& q_at) {
       constexpr int kLanes = D / 8, kRows = 32 / kLanes;  // per copy
       const int fr = q_at.tile * kTile + st * kRowsPerStream + row;
-      const int t = fr / p.group, head = q_at.head * p.group + fr - t * p.group;
+      const int t = p.by_group(fr), head = q_at.head * p.group + fr - t * p.group;
       const bool live = fr < q_at.req.qlen * p.group;
       const int64_t off = live ? (q_at.req.q0 + t) * p.q_token_stride + head * p.q_head_stride : -1;
       const int ch = lane % kLanes, first = (warp & 3) * 32 + lane / kLanes;
@@ -428,15 +422,15 @@ __global__ void __launch_bounds__(kThreads, 1)
       const int rows = at.req.qlen * p.group, cached = at.req.seq - at.req.qlen;
       const int fr = at.tile * kTile + st * kRowsPerStream + row;  // flattened row
       const bool live = fr < rows;
-      const int t = fr / p.group, head = at.head * p.group + fr - t * p.group;
+      const int t = p.by_group(fr), head = at.head * p.group + fr - t * p.group;
       float m = -INFINITY, l = 0.f;
       if (r.active) {
         // keys (j > low, j <= high) of this row, and those that all of the warp's rows see
         const int high = live ? cached + t : -1;
         const int low = p.window > 0 ? cached + t - p.window : -1;
         const int f_row = at.tile * kTile + st * kRowsPerStream + (row & ~31);
-        const int high_min = cached + f_row / p.group;
-        const int low_max = p.window > 0 ? cached + (min(f_row + 32, rows) - 1) / p.group - p.window : -1;
+        const int high_min = cached + p.by_group(f_row);
+        const int low_max = p.window > 0 ? cached + p.by_group(min(f_row + 32, rows) - 1) - p.window : -1;
         for (int blk = r.begin; blk < r.end; ++blk) {
           mbar_wait_bounded(&c.s_full[st], s_phase, p.err, abort_flag);
           s_phase ^= 1u;
