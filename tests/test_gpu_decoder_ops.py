@@ -702,3 +702,36 @@ def test_attention_work_cut_anywhere(cuda, B, new):
     for top in (130, 700, 3000 if B < 100 else 1300):
         _attention_case(cuda, [(rng.randint(0, top), rng.randint(1, new)) for _ in range(B)], 8, 1, 64, 16,
                         workspace=ws, seed=top)
+
+
+def _keyless_runs(rng, B, run, top):
+    """Single tokens over 1 .. top keys, with runs of requests without any at the front, in the middle and
+    at the end, and further runs of other lengths between them."""
+    lens = [(rng.randint(1, top), 1) for _ in range(B)]
+    for at in (0, B // 2, B - run, B // 5, B // 3 + 1):
+        lens[at:at + run] = [(0, 1)] * run
+    for at in range(B // 2 + 20, B - 20, 11):
+        n = rng.randint(1, 9)
+        lens[at:at + n] = [(0, 1)] * n
+    return lens
+
+
+@pytest.mark.parametrize("run", [1, 2, 9])
+@pytest.mark.parametrize("Hkv", [8, 4, 2, 1])
+def test_attention_requests_without_keys_among_others(cuda, Hkv, run):
+    """Padded rows of a decode batch: their segments take no turn of the query ring."""
+    rng = random.Random(Hkv * 10 + run)
+    _, ws = _attention_case(cuda, _keyless_runs(rng, 512, run, 500), 2 * Hkv, Hkv, 64, 16)
+    one = [(500, 1)] * 512
+    one[:run] = [(0, 1)] * run
+    _attention_case(cuda, one, Hkv, Hkv, 64, 16, workspace=ws)
+
+
+def test_attention_requests_without_keys_in_long_and_mixed_batches(cuda):
+    rng = random.Random(1)
+    _, ws = _attention_case(cuda, _keyless_runs(rng, 3000, 4, 60), 4, 2, 128, 16)
+    _attention_case(cuda, _keyless_runs(rng, 600, 3, 2500), 4, 4, 64, 64, workspace=ws)
+    # beside the tensor-core kernel, whose own requests have some without keys, too
+    lens = _keyless_runs(rng, 400, 3, 700) + [(700, 200), (0, 50), (3, 90), (0, 200)]
+    rng.shuffle(lens)
+    _attention_case(cuda, lens, 8, 4, 64, 16, workspace=ws)

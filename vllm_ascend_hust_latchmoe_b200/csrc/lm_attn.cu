@@ -15,6 +15,7 @@
 #include <string>
 
 #include "lm_attn.cuh"
+#include "lm_attn_ring.cuh"
 #include "lm_tmap.cuh"
 
 namespace lm {
@@ -146,12 +147,14 @@ __global__ void __launch_bounds__(kThreads, 1)
   }
   if (warp > kWarps) {
     // ------------------------------------------------------------------------ queries
-    for (int seg = 0; attn_has<kItem>(at, w, w_end); ++seg) {
+    AttnQueryTurn turn;
+    while (attn_has<kItem>(at, w, w_end)) {
       const AttnSegment s = attn_segment<kTileRows, kBlock, kItem>(p, at, w, w_end);
-      if (s.blk1 > s.blk0) {
-        if (!warp_wait(&c.q_empty[seg & 1], ((seg >> 1) & 1) ^ 1u, p.err, abort_flag)) break;
+      if (turn.has_keys(s.blk0, s.blk1)) {
+        const int buf = turn.buffer();
+        if (!warp_wait(&c.q_empty[buf], turn.empty_parity(), p.err, abort_flag)) break;
         const int rows = at.req.qlen * p.group;
-        unsigned char* dst = s_q + (seg & 1) * S::kQ;
+        unsigned char* dst = s_q + buf * S::kQ;
 #pragma unroll
         for (int j = 0; j < kTileRows * kChunks / 32; ++j) {
           const int r = (j * 32 + lane) / kChunks, ch = (j * 32 + lane) % kChunks;
@@ -160,7 +163,8 @@ __global__ void __launch_bounds__(kThreads, 1)
           const uint16_t* src = p.q + (at.req.q0 + t) * p.q_token_stride + head * p.q_head_stride + ch * 8;
           cp_async_16(dst + q_at<D>(r, ch), row < rows ? src : p.q, row < rows ? 16u : 0u);
         }
-        cp_async_arrive_noinc(&c.q_full[seg & 1]);
+        cp_async_arrive_noinc(&c.q_full[buf]);
+        turn.next();
       }
       w += s.units;
       if (w >= w_end) break;
@@ -176,7 +180,8 @@ __global__ void __launch_bounds__(kThreads, 1)
   // whatever their stages hold (every later wait returns at once), so that their barriers match.
   const int g = lane >> 2, c2 = (lane & 3) * 2;
   int seq = 0;
-  for (int seg = 0; attn_has<kItem>(at, w, w_end); ++seg) {
+  AttnQueryTurn turn;
+  while (attn_has<kItem>(at, w, w_end)) {
     const AttnSegment s = attn_segment<kTileRows, kBlock, kItem>(p, at, w, w_end);
     const int rows = at.req.qlen * p.group;
     const int row_base = at.tile * kTileRows;
@@ -184,17 +189,17 @@ __global__ void __launch_bounds__(kThreads, 1)
     const int n_slices = s.blk1 - s.blk0;  // one slice of this warp per block
 
     uint32_t qf[D / 16][4];
-    if (n_slices > 0) {
-      mbar_wait_bounded(&c.q_full[seg & 1], (seg >> 1) & 1, p.err, abort_flag);
-      const uint32_t qa = smem_u32(s_q + (seg & 1) * S::kQ);
+    if (turn.has_keys(s.blk0, s.blk1)) {
+      const int buf = turn.buffer();
+      mbar_wait_bounded(&c.q_full[buf], turn.full_parity(), p.err, abort_flag);
+      const uint32_t qa = smem_u32(s_q + buf * S::kQ);
 #pragma unroll
       for (int k = 0; k < D / 16; ++k)  // rows 0-7, 8-15, then the same 8 columns on
         ldmatrix_x4(qf[k], qa + q_at<D>(lane & 15, 2 * k + (lane >> 4)));
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&c.q_empty[buf]);
+      turn.next();
     }
-    __syncwarp();
-    // a segment without keys passes its turn, so that the parities stay with the segment number
-    if (lane == 0) mbar_arrive(&c.q_empty[seg & 1]);
-    if (n_slices == 0 && warp == 0) cp_async_arrive_noinc(&c.q_full[seg & 1]);
 
     // keys (j > low, j <= high) that rows g and g + 8 of the tile see
     const int r0 = row_base + g, r1 = r0 + 8;
