@@ -12,6 +12,9 @@ largest score error), and the exponentials and the logarithm 2^-20 of 1 + |lse|.
 
 import math
 import random
+import subprocess
+import sys
+from pathlib import Path
 
 import pytest
 import torch
@@ -21,6 +24,7 @@ from vllm_ascend_hust_latchmoe_b200 import decoder_ops as ops
 
 pytestmark = pytest.mark.gpu
 
+ROOT = Path(__file__).resolve().parents[1]
 BF16 = 2.0 ** -8
 SUMS = 1e-5
 
@@ -735,3 +739,13 @@ def test_attention_requests_without_keys_in_long_and_mixed_batches(cuda):
     lens = _keyless_runs(rng, 400, 3, 700) + [(700, 200), (0, 50), (3, 90), (0, 200)]
     rng.shuffle(lens)
     _attention_case(cuda, lens, 8, 4, 64, 16, workspace=ws)
+
+
+def test_page_tables_of_any_number_of_requests(cuda):
+    """Counts around the one whose shared memory, static part included, passes 48 KB: in a process of
+    their own, since a larger call before them would have raised the kernel's limit."""
+    code = ("import torch, tests.test_gpu_decoder_ops as t\n"
+            "for B in (4052, 4053, 4054, 4095, 4096):\n"
+            "    t._tables_case(torch.device('cuda', 0), [3] * B, [1] * (B - 1) + [40], 16, 4)\n")
+    done = subprocess.run([sys.executable, "-c", code], cwd=ROOT, capture_output=True, text=True, timeout=300)
+    assert done.returncode == 0, done.stderr[-2000:]

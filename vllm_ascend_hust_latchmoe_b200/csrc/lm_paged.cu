@@ -15,6 +15,7 @@ constexpr int kTableThreads = 1024;
 constexpr int kTableCtas = 8;  // one cluster, so that its barrier orders reads before writes
 constexpr int kMaxRequests = 4096;
 constexpr int kPerThread = kMaxRequests / kTableThreads;
+constexpr size_t kTableStatic = 1024;  // at least page_tables_kernel's static shared memory (516 bytes)
 
 struct TableParams {
   const int32_t* cached;
@@ -582,7 +583,8 @@ extern "C" int lm_build_page_tables(const int32_t* cached_lens, const int32_t* n
                       num_requests, page_size, max_pages, free_capacity,
                       ((reinterpret_cast<uintptr_t>(positions) | reinterpret_cast<uintptr_t>(slot_mapping)) & 15) == 0};
   const size_t smem = (3 * static_cast<size_t>(num_requests) + 1) * 4;
-  if (smem > 48 * 1024) {
+  // Without the opt-in static and dynamic shared memory together have 48 KB.
+  if (smem + kTableStatic > 48 * 1024) {
     const int rc = check_cuda(cudaFuncSetAttribute(page_tables_kernel,
                                                    cudaFuncAttributeMaxDynamicSharedMemorySize,
                                                    (3 * kMaxRequests + 1) * 4),
