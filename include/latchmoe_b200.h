@@ -510,7 +510,9 @@ int lm_add_rms_norm(const uint16_t* x, int64_t x_stride, const uint16_t* residua
  * a call with other outputs changes nothing that it reads, so it may be repeated.
  * A row without enough free pages or table columns gets none (LM_DEVERR_NO_PAGES): its tokens have
  * slot -1 and its sequence length stays; so do all rows behind it that need a page, if the stack
- * ran out. A bad length counts as 0 (LM_DEVERR_BAD_LENGTH), tokens past max_tokens are cut. */
+ * ran out. A bad length (below 0, cached past the row's pages, new past max_tokens) counts as 0, and
+ * tokens past max_tokens are cut off new_lens, with no place, no page and no part of seq_lens (both
+ * LM_DEVERR_BAD_LENGTH). */
 int lm_build_page_tables(const int32_t* cached_lens, const int32_t* new_lens,
                          int32_t num_requests, int32_t page_size, int32_t* block_tables,
                          int64_t table_stride, int32_t max_pages, const int32_t* free_pages,

@@ -749,3 +749,46 @@ def test_page_tables_of_any_number_of_requests(cuda):
             "    t._tables_case(torch.device('cuda', 0), [3] * B, [1] * (B - 1) + [40], 16, 4)\n")
     done = subprocess.run([sys.executable, "-c", code], cwd=ROOT, capture_output=True, text=True, timeout=300)
     assert done.returncode == 0, done.stderr[-2000:]
+
+
+@pytest.mark.parametrize("cached,new,T,page", [
+    ([5, 0, 30], [20, 24, 3], 25, 16),  # the second request keeps 5 tokens, the third none
+    ([0, 0, 0], [40, 40, 9], 42, 16),  # the second request's first page, none for the third
+    ([0, 0], [40, 40], 0, 16),
+    ([16] * 1100, [9] * 1100, 5003, 16),  # several blocks
+    ([7] * 4096, [3] * 4096, 6001, 1)])
+@pytest.mark.parametrize("in_place", [False, True])
+def test_page_tables_cut_tokens_hold_no_pages(cuda, cached, new, T, page, in_place):
+    """A step with more tokens than its buffers hold gives what the step of the tokens that fit would give."""
+    B, room, kept = len(cached), T, []
+    for n in new:
+        kept.append(min(n, room))
+        room -= kept[-1]
+    width = max(1, -(-max(c + n for c, n in zip(cached, kept)) // page))  # too narrow for some of the cut rows
+    have = [-(-c // page) for c in cached]
+    grants = sum(-(-(c + n) // page) - h for c, n, h in zip(cached, kept, have))
+    pool = list(range(sum(have) + grants))  # and no page more than the kept tokens need
+    random.Random(T).shuffle(pool)
+    tables, at = [[-1] * width for _ in range(B)], 0
+    for b, h in enumerate(have):
+        tables[b][:h] = pool[at:at + h]
+        at += h
+    free = pool[at:]
+
+    def ints(v, dtype=torch.int32):
+        return torch.tensor(v, dtype=dtype, device=cuda)
+
+    dt, lens, dfree, count, err = ints(tables), ints(cached), ints(free + [-7]), ints([len(free)]), ints([0])
+    seq = lens if in_place else ints([-5] * B)
+    left = count if in_place else ints([-5])
+    cu, pos, slots = ints([-5] * (B + 1)), ints([-5] * T), ints([-5] * T, torch.int64)
+    ops.build_page_tables(lens, ints(new), page, dt, dfree, count, seq_lens=seq, cu_q=cu, positions=pos,
+                          slot_mapping=slots, free_count_out=left, err_word=err)
+    want = _tables_by_hand(cached, kept, page, tables, free, len(free), T)
+    assert (seq.tolist(), cu.tolist(), pos.tolist(), slots.tolist(), left.item()) == want[:5]
+    assert dt.tolist() == tables and err.item() == 6
+    if in_place:  # every page comes back
+        ops.release_pages(torch.arange(B, dtype=torch.int32, device=cuda), lens, page, dt,
+                          (every := ints([-1] * (len(pool) + 1))), (n := ints([0])))
+        assert n.item() == len(pool) - left.item() == sum(have) + grants
+        assert sorted(every.tolist()) == sorted(pool + [-1])

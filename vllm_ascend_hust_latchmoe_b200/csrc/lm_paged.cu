@@ -151,6 +151,12 @@ __global__ void __launch_bounds__(kTableThreads) page_tables_kernel(const TableP
     if (threadIdx.x == 0) record_error(p.err, LM_DEVERR_BAD_LENGTH);
     free_count = min(max(free_count, 0), p.free_capacity);
   }
+  const int64_t limit = static_cast<int64_t>(p.max_pages) * page;
+  // pages that n tokens behind c cached ones need, or why they get none
+  constexpr int kBadLength = -1, kNoRoom = -2;
+  auto pages_for = [&](int c, int n) {
+    return static_cast<int64_t>(c) + n > limit ? kNoRoom : (c + n + page - 1) / page - (c + page - 1) / page;
+  };
   int need[kPerThread], fresh[kPerThread], cached[kPerThread];
   int64_t sum_need = 0, sum_fresh = 0;
 #pragma unroll
@@ -160,7 +166,6 @@ __global__ void __launch_bounds__(kTableThreads) page_tables_kernel(const TableP
     if (i >= per || b >= B) continue;
     cached[i] = p.cached[b];
     fresh[i] = p.fresh[b];
-    const int64_t limit = static_cast<int64_t>(p.max_pages) * page;
     bool bad = false;
     if (cached[i] < 0 || cached[i] > limit) {
       bad = true;
@@ -170,28 +175,39 @@ __global__ void __launch_bounds__(kTableThreads) page_tables_kernel(const TableP
       bad = true;
       fresh[i] = 0;
     }
-    if (bad) {
-      record_error(p.err, LM_DEVERR_BAD_LENGTH);
-      need[i] = -1;
-    } else if (static_cast<int64_t>(cached[i]) + fresh[i] > limit) {
-      record_error(p.err, LM_DEVERR_NO_PAGES);
-      need[i] = -1;
-    } else {
-      need[i] = (cached[i] + fresh[i] + page - 1) / page - (cached[i] + page - 1) / page;
-    }
+    if (bad) record_error(p.err, LM_DEVERR_BAD_LENGTH);
+    need[i] = bad ? kBadLength : pages_for(cached[i], fresh[i]);
     sum_need += max(need[i], 0);
     sum_fresh += fresh[i];
   }
   int64_t at_need = sum_need, at_fresh = sum_fresh, total_need, total_fresh;
   block_scan2(at_need, at_fresh, total_need, total_fresh, s_warp);
+  if (total_fresh > p.max_tokens) {  // the tokens are cut, and pages are for those that are left
+    if (threadIdx.x == 0) record_error(p.err, LM_DEVERR_BAD_LENGTH);
+    int64_t first = at_fresh;
+    sum_need = sum_fresh = 0;
+#pragma unroll
+    for (int i = 0; i < kPerThread; ++i) {
+      const int left = static_cast<int>(max(p.max_tokens - first, int64_t{0}));
+      first += fresh[i];
+      fresh[i] = min(fresh[i], left);
+      if (need[i] != kBadLength) need[i] = pages_for(cached[i], fresh[i]);
+      sum_need += max(need[i], 0);
+      sum_fresh += fresh[i];
+    }
+    at_need = sum_need;
+    at_fresh = sum_fresh;
+    __syncthreads();  // s_warp has been read
+    block_scan2(at_need, at_fresh, total_need, total_fresh, s_warp);
+  }
   int granted = 0;  // pages up to and including this thread's last request that got its pages
 #pragma unroll
   for (int i = 0; i < kPerThread; ++i) {
     const int b = threadIdx.x * per + i;
     if (i >= per || b >= B) continue;
-    s_cu[b] = static_cast<int32_t>(min(at_fresh, p.max_tokens));
+    s_cu[b] = static_cast<int32_t>(at_fresh);
     bool ok = need[i] >= 0;
-    if (ok && need[i] > 0 && at_need + need[i] > free_count) {
+    if (need[i] == kNoRoom || (need[i] > 0 && at_need + need[i] > free_count)) {
       record_error(p.err, LM_DEVERR_NO_PAGES);
       ok = false;
     }
@@ -201,10 +217,7 @@ __global__ void __launch_bounds__(kTableThreads) page_tables_kernel(const TableP
     at_need += max(need[i], 0);
     at_fresh += fresh[i];
   }
-  if (threadIdx.x == 0) {
-    s_cu[B] = static_cast<int32_t>(min(total_fresh, p.max_tokens));
-    if (total_fresh > p.max_tokens) record_error(p.err, LM_DEVERR_BAD_LENGTH);
-  }
+  if (threadIdx.x == 0) s_cu[B] = static_cast<int32_t>(total_fresh);
   // The largest grant ends the pages taken: requests are granted in order, and once one does not
   // fit, every later one that needs a page does not either.
   if (granted > 0) atomicMax(&s_used, granted);
