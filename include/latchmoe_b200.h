@@ -522,8 +522,9 @@ int lm_build_page_tables(const int32_t* cached_lens, const int32_t* new_lens,
                          int32_t* err_word, void* stream);
 
 /* The pages of the listed rows (ceil(cached_lens / page_size) entries each) go back onto the free
- * stack in the order of the list; their table entries become -1 and their lengths 0. A row outside
- * the table or a stack overflow is recorded (LM_DEVERR_BAD_LENGTH) and skipped. */
+ * stack in the order of the list; their table entries become -1 and their lengths 0. Entries below 0
+ * (pages given back before, as behind a sliding window) are passed over. A row outside the table or a
+ * stack overflow is recorded (LM_DEVERR_BAD_LENGTH) and skipped. */
 int lm_release_pages(const int32_t* rows, int32_t num_rows, int32_t* cached_lens,
                      int32_t num_requests, int32_t page_size, int32_t* block_tables,
                      int64_t table_stride, int32_t max_pages, int32_t* free_pages,

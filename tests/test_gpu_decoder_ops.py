@@ -792,3 +792,30 @@ def test_page_tables_cut_tokens_hold_no_pages(cuda, cached, new, T, page, in_pla
                           (every := ints([-1] * (len(pool) + 1))), (n := ints([0])))
         assert n.item() == len(pool) - left.item() == sum(have) + grants
         assert sorted(every.tolist()) == sorted(pool + [-1])
+
+
+def test_release_pages_passes_over_entries_without_a_page(cuda):
+    """Pages that left a window were given back already: their entries are negative."""
+    def ints(v, dtype=torch.int32):
+        return torch.tensor(v, dtype=dtype, device=cuda)
+
+    tables, lens = ints([[-1, -1, 7], [4, 5, -1], [-1, 9, -1]]), ints([48, 20, 33])
+    free, count, err = ints([0, -8, -8, -8, -8]), ints([1]), ints([0])
+    ops.release_pages(ints([0, 2, 1]), lens, 16, tables, free, count, err)
+    assert free.tolist() == [0, 7, 9, 4, 5] and count.item() == 5 and err.item() == 0
+    assert lens.tolist() == [0, 0, 0] and tables.tolist() == [[-1] * 3] * 3
+    # long rows, more entries than the stack has room for and just as many pages
+    rng = random.Random(4)
+    rows = [[rng.choice([-1, -1, b * 1000 + i]) for i in range(700)] for b in range(3)]
+    want = [i for b in (2, 0, 1) for i in rows[b][:620] if i >= 0]
+    tables, lens = ints(rows), ints([620] * 3)
+    free, count = ints([-8] * (len(want) + 1)), ints([0])
+    ops.release_pages(ints([2, 0, 1]), lens, 1, tables, free, count, err)
+    assert free.tolist() == want + [-8] and count.item() == len(want) and err.item() == 0
+    assert tables.tolist() == [[-1] * 620 + r[620:] for r in rows]
+    # a page too many: the row stays as it is, the others go back
+    tables, lens = ints([[1, -1, 2], [3, 4, 5]]), ints([3, 3])
+    free, count = ints([-8] * 4), ints([0])
+    ops.release_pages(ints([0, 1]), lens, 1, tables, free, count, err)
+    assert free.tolist() == [1, 2, -8, -8] and count.item() == 2 and err.item() == 6
+    assert lens.tolist() == [0, 3] and tables.tolist() == [[-1] * 3, [3, 4, 5]]

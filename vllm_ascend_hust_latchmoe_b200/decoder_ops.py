@@ -87,7 +87,8 @@ def release_pages(rows: torch.Tensor, cached_lens: torch.Tensor, page_size: int,
                   block_tables: torch.Tensor, free_pages: torch.Tensor, free_count: torch.Tensor,
                   err_word: torch.Tensor | None = None) -> None:
     """Give the pages of the requests in ``rows`` (int32) back: they go onto the free stack, their
-    table entries become -1 and their ``cached_lens`` 0."""
+    table entries become -1 and their ``cached_lens`` 0. Entries below 0 (pages that were given back
+    before, as behind a sliding window) are passed over."""
     (_binding or _load()).release_pages(rows, cached_lens, page_size, block_tables, free_pages,
                                         free_count, err_word)
 
