@@ -819,3 +819,13 @@ def test_release_pages_passes_over_entries_without_a_page(cuda):
     ops.release_pages(ints([0, 1]), lens, 1, tables, free, count, err)
     assert free.tolist() == [1, 2, -8, -8] and count.item() == 2 and err.item() == 6
     assert lens.tolist() == [0, 3] and tables.tolist() == [[-1] * 3, [3, 4, 5]]
+
+
+@pytest.mark.parametrize("window", [2 ** 31 - 1, 2 ** 31 - 5, 2 ** 30])
+@pytest.mark.parametrize("Hq,Hkv,D", [(8, 1, 128), (2, 2, 64)])
+def test_attention_window_past_every_key(cuda, Hq, Hkv, D, window):
+    """Windows that stand for none, also where the first queries come before every key; both kernels."""
+    for max_q in (1, 1000):
+        _attention_case(cuda, [(2, 6), (5, 5), (0, 3), (1, 1), (300, 1)], Hq, Hkv, D, 16, window=window,
+                        max_q=max_q)
+    _attention_case(cuda, [(2, 6), (150, 400), (300, 300), (0, 300), (700, 1)], Hq, Hkv, D, 16, window=window)

@@ -206,8 +206,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     const int t0 = p.by_group(r0), t1 = p.by_group(r1);
     const int high0 = r0 < rows ? cached + t0 : -1;
     const int high1 = r1 < rows ? cached + t1 : -1;
-    const int low0 = p.window > 0 ? cached + t0 - p.window : -1;
-    const int low1 = p.window > 0 ? cached + t1 - p.window : -1;
+    const int low0 = attn_hidden(p, cached + t0), low1 = attn_hidden(p, cached + t1);
 
     float o[D / 8][4];
 #pragma unroll

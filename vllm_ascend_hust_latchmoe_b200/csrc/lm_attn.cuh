@@ -87,6 +87,12 @@ __device__ __forceinline__ AttnRequest attn_request(const AttnParams& p, int b, 
   return r;
 }
 
+// The last key that a window hides from a row at position `pos`, -1 for none. (Rows before every key have
+// negative positions, see nothing and may name any key here; a window of up to 2^31 - 1 must not wrap.)
+__device__ __forceinline__ int attn_hidden(const AttnParams& p, int pos) {
+  return p.window > 0 ? max(pos, 0) - p.window : -1;
+}
+
 // Keys that some row of tile `tile` sees: [lo, hi).
 template <int TILE_ROWS>
 __device__ __forceinline__ void attn_tile_keys(const AttnParams& p, const AttnRequest& r, int tile,
@@ -96,7 +102,7 @@ __device__ __forceinline__ void attn_tile_keys(const AttnParams& p, const AttnRe
   const int last = p.by_group(min((tile + 1) * TILE_ROWS, rows) - 1);
   const int cached = r.seq - r.qlen;  // negative: the first queries stand before every key
   hi = max(0, cached + last + 1);
-  lo = p.window > 0 ? min(hi, max(0, cached + first - p.window + 1)) : 0;
+  lo = min(hi, max(0, attn_hidden(p, cached + first) + 1));
 }
 
 template <int BLOCK>

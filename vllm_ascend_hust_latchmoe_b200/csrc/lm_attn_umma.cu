@@ -427,10 +427,10 @@ __global__ void __launch_bounds__(kThreads, 1)
       if (r.active) {
         // keys (j > low, j <= high) of this row, and those that all of the warp's rows see
         const int high = live ? cached + t : -1;
-        const int low = p.window > 0 ? cached + t - p.window : -1;
+        const int low = attn_hidden(p, cached + t);
         const int f_row = at.tile * kTile + st * kRowsPerStream + (row & ~31);
         const int high_min = cached + p.by_group(f_row);
-        const int low_max = p.window > 0 ? cached + p.by_group(min(f_row + 32, rows) - 1) - p.window : -1;
+        const int low_max = attn_hidden(p, cached + p.by_group(min(f_row + 32, rows) - 1));
         for (int blk = r.begin; blk < r.end; ++blk) {
           mbar_wait_bounded(&c.s_full[st], s_phase, p.err, abort_flag);
           s_phase ^= 1u;
