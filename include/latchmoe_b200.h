@@ -563,7 +563,9 @@ int lm_rope_cache_write(const uint16_t* qkv, int64_t qkv_stride, const int32_t* 
  * kernels; results do not depend on it being right. The workspace
  * (lm_paged_attention_workspace_bytes() for the current device, 16-byte aligned, zeroed once) is
  * left ready for the next call; calls that share one must not overlap. A table entry outside the
- * cache is recorded (LM_DEVERR_BAD_PAGE) and its keys count as zeros. */
+ * cache is recorded (LM_DEVERR_BAD_PAGE) and its keys count as zeros. A query range that is not inside
+ * [0, num_tokens] counts as empty and a length outside its table row is held to it (LM_DEVERR_BAD_LENGTH);
+ * where ranges overlap so much that their work passes 32-bit counts, nothing is computed (the same). */
 int64_t lm_paged_attention_workspace_bytes(void);
 int lm_paged_attention(const uint16_t* q, int64_t q_token_stride, int64_t q_head_stride,
                        const uint16_t* k_cache, int64_t k_page_stride, int64_t k_token_stride,

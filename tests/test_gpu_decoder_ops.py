@@ -829,3 +829,22 @@ def test_attention_window_past_every_key(cuda, Hq, Hkv, D, window):
         _attention_case(cuda, [(2, 6), (5, 5), (0, 3), (1, 1), (300, 1)], Hq, Hkv, D, 16, window=window,
                         max_q=max_q)
     _attention_case(cuda, [(2, 6), (150, 400), (300, 300), (0, 300), (700, 1)], Hq, Hkv, D, 16, window=window)
+
+
+@pytest.mark.parametrize("B,T,page,hint", [
+    (4096, 1024, 1024, 1024), (4096, 1024, 1024, 1), (32, 20480, 4096, 20480), (32, 16384, 1024, 0)])
+def test_attention_overlapping_query_ranges_do_not_wrap_the_units(cuda, B, T, page, hint):
+    """Every other range takes all tokens again, over a million keys each: more units in all than 32 bits
+    count, though no request for itself has. Nothing is computed, and the error says so."""
+    g = _gen(cuda, 6)
+    kc, q = _bf16(g, 1, page, 1, 64), _bf16(g, T, 64, 64)
+    width = 1024
+    tables = torch.zeros(B, width, dtype=torch.int32, device=cuda)
+    seq = torch.full((B,), width * page, dtype=torch.int32, device=cuda)
+    cu = torch.tensor([0, T] * (B // 2) + [0], dtype=torch.int32, device=cuda)
+    out, lse = torch.full_like(q, 7.0), torch.full((T, 64), 7.0, device=cuda)
+    err = torch.zeros(1, dtype=torch.int32, device=cuda)
+    ws = ops.attention_workspace(cuda)
+    ops.paged_attention(q, kc, kc, tables, seq, cu, out, max_q_len=hint, workspace=ws, lse=lse, err_word=err)
+    assert err.item() == 6 and (out == 7.0).all() and (lse == 7.0).all()
+    assert (ws == 0).all()  # and the workspace is as a call needs it

@@ -549,7 +549,7 @@ extern "C" int lm_paged_attention(
   if (page_size <= 0 || page_size % 16 != 0)
     return fail(LM_ERR_INVALID_ARGUMENT, "lm_paged_attention: page_size must be a multiple of 16");
   if (num_requests < 0 || num_requests > kAttnMaxRequests || num_tokens < 0 ||
-      num_tokens * num_q_heads > 0x7fffffff || num_pages < 0 || num_pages > 0x7fffffff ||
+      num_tokens > 0x7fffffff || num_tokens * num_q_heads > 0x7fffffff - kAttnMaxPartialRows || num_pages < 0 || num_pages > 0x7fffffff ||
       max_pages <= 0 || table_stride < max_pages || max_q_len < 0 || window < 0 ||
       static_cast<int64_t>(max_pages) * page_size > 0x7fffffff - 128)
     return fail(LM_ERR_INVALID_ARGUMENT, "lm_paged_attention: bad sizes (at most 4096 requests)");
@@ -560,7 +560,7 @@ extern "C" int lm_paged_attention(
     const int64_t tiles = num_tokens * num_q_heads / (small ? kTileRows : 2 * 128) +
                           static_cast<int64_t>(num_requests) * num_kv_heads;
     const int64_t blocks = (static_cast<int64_t>(max_pages) * page_size + kBlock - 1) / kBlock + 1 + 3;
-    if (tiles > 0x7fffffff / blocks)
+    if (tiles > (kAttnMaxUnits - 1) / blocks)
       return fail(LM_ERR_UNSUPPORTED, "lm_paged_attention: too much work for one call");
   }
   if (q == nullptr || k_cache == nullptr || v_cache == nullptr || block_tables == nullptr ||

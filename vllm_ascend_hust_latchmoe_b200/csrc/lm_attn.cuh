@@ -21,6 +21,14 @@ namespace lm {
 constexpr int kAttnMaxRequests = 4096;
 constexpr int kAttnMaxCtas = 512;      // counters in the workspace
 constexpr int kAttnMaxPartialRows = 256;
+constexpr int kAttnMaxUnits = 0x7fff0000;  // of a launch; the rest of 32 bits is for a CTA's share past them
+
+// Sum of two counts of units, at most kAttnMaxUnits. One request's units fit (the host has seen to it), and
+// those of query ranges that follow each other do as well, but ranges on the device may overlap.
+__device__ __forceinline__ int attn_add(int a, int b) {
+  return static_cast<int>(min(static_cast<uint32_t>(a) + static_cast<uint32_t>(b),
+                              static_cast<uint32_t>(kAttnMaxUnits)));
+}
 
 // n / d for 0 <= n < 2^31 as a product and a shift: mul = ceil(2^shift / d) with shift = 31 +
 // ceil(log2 d) is above 2^shift / d by less than 2^(shift - 31) / d, which n is too small to show.
@@ -170,22 +178,22 @@ __device__ __forceinline__ void attn_prefix(const AttnParams& p, int32_t* s_pref
     }
     const int cost = attn_cost<TILE_ROWS, BLOCK, ITEM>(p, r, tiles, longest);
     if (b < b1) s_prefix[b + 1] = cost * p.kv_heads;
-    sum += cost * p.kv_heads;
+    sum = attn_add(sum, cost * p.kv_heads);
   }
   int incl = sum;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
 #pragma unroll
   for (int o = 1; o < 32; o <<= 1) {
     const int u = __shfl_up_sync(0xffffffffu, incl, o);
-    if (lane >= o) incl += u;
+    if (lane >= o) incl = attn_add(incl, u);
   }
   if (lane == 31) s_warp[warp] = incl;
   atomicMax(s_longest, longest);
   __syncthreads();
   int base = incl - sum;
-  for (int w = 0; w < warp; ++w) base += s_warp[w];
+  for (int w = 0; w < warp; ++w) base = attn_add(base, s_warp[w]);
   for (int b = b0; b < b1; ++b) {
-    base += s_prefix[b + 1];
+    base = attn_add(base, s_prefix[b + 1]);
     s_prefix[b + 1] = base;
   }
   if (threadIdx.x == 0) s_prefix[0] = 0;
@@ -259,13 +267,17 @@ __device__ __forceinline__ bool attn_locate(const AttnParams& p, int32_t* s_pref
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
       const int u = __shfl_up_sync(0xffffffffu, incl, o);
-      if (lane >= o) incl += u;
+      if (lane >= o) incl = attn_add(incl, u);
     }
     total = __shfl_sync(0xffffffffu, incl, 31);
   } else {
     attn_prefix<TILE_ROWS, BLOCK, ITEM, NT>(p, s_prefix, s_warp, s_longest);
     total = s_prefix[B];
     longest = *s_longest;
+  }
+  if (total == kAttnMaxUnits) {  // more than can be told apart: nothing is computed
+    if (blockIdx.x == 0 && threadIdx.x == 0) record_error(p.err, LM_DEVERR_BAD_LENGTH);
+    return false;
   }
   const int fewest = FEW && longest > 8 ? static_cast<int>(sqrtf(static_cast<float>(longest))) : 1;
   per = max(fewest, (total + static_cast<int>(gridDim.x) - 1) / static_cast<int>(gridDim.x));
