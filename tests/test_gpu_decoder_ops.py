@@ -848,3 +848,15 @@ def test_attention_overlapping_query_ranges_do_not_wrap_the_units(cuda, B, T, pa
     ops.paged_attention(q, kc, kc, tables, seq, cu, out, max_q_len=hint, workspace=ws, lse=lse, err_word=err)
     assert err.item() == 6 and (out == 7.0).all() and (lse == 7.0).all()
     assert (ws == 0).all()  # and the workspace is as a call needs it
+
+
+def test_page_tables_pages_near_2_31_tokens(cuda):
+    """Tokens + page size past 2^31 (tables alone: no cache has such pages)."""
+    for page in (2 ** 31 - 1, 2 ** 30):
+        _tables_case(cuda, [5, 0, page - 60, page, 0], [1, 3, 50, 0, 0], page, 1)
+        _tables_case(cuda, [5, page - 60], [3000, 50], page, 1, pad=2000, in_place=True)
+    _tables_case(cuda, [2 ** 30 - 1, 2 ** 30 - 20], [2, 9], 2 ** 30 - 1, 2)
+    one = dict(dtype=torch.int32, device=cuda)
+    tables, lens, free, count = (torch.tensor(v, **one) for v in ([[3]], [2 ** 31 - 2], [-8, -8], [0]))
+    ops.release_pages(torch.zeros(1, **one), lens, 2 ** 31 - 1, tables, free, count)
+    assert free.tolist() == [3, -8] and count.item() == 1 and lens.item() == 0 and tables.item() == -1

@@ -73,6 +73,12 @@ __device__ __forceinline__ void block_scan2(int64_t& a, int64_t& b, int64_t& tot
   b = ib - b + (warp ? s_warp[warp - 1][1] : 0);
 }
 
+// Pages of `tokens` tokens; unsigned, as the sum may pass 2^31 where a page is about as long.
+__device__ __forceinline__ int pages_of(int tokens, int page) {
+  return static_cast<int>((static_cast<uint32_t>(tokens) + static_cast<uint32_t>(page) - 1u) /
+                          static_cast<uint32_t>(page));
+}
+
 // The last of n ascending values that is at most x (values[0] is).
 __device__ __forceinline__ int last_at_most(const int32_t* values, int n, int64_t x) {
   int lo = 0, hi = n;
@@ -104,7 +110,7 @@ __device__ __forceinline__ void place_tokens(const TableParams& p, const int32_t
       const int kept = s_cached[lo], c = kept < 0 ? ~kept : kept;
       pos[e] = c + static_cast<int>(t) - s_cu[lo];
       if (kept < 0) continue;
-      const int have = (c + page - 1) / page, i = pos[e] / page;
+      const int have = pages_of(c, page), i = pos[e] / page;
       // pages already held are read from the table, granted ones from the stack (another CTA may be
       // writing their table entries)
       const int id = i < have ? p.tables[lo * p.table_stride + i]
@@ -155,7 +161,7 @@ __global__ void __launch_bounds__(kTableThreads) page_tables_kernel(const TableP
   // pages that n tokens behind c cached ones need, or why they get none
   constexpr int kBadLength = -1, kNoRoom = -2;
   auto pages_for = [&](int c, int n) {
-    return static_cast<int64_t>(c) + n > limit ? kNoRoom : (c + n + page - 1) / page - (c + page - 1) / page;
+    return static_cast<int64_t>(c) + n > limit ? kNoRoom : pages_of(c + n, page) - pages_of(c, page);
   };
   int need[kPerThread], fresh[kPerThread], cached[kPerThread];
   int64_t sum_need = 0, sum_fresh = 0;
@@ -229,7 +235,7 @@ __global__ void __launch_bounds__(kTableThreads) page_tables_kernel(const TableP
   // new table entries: a thread per granted page
   for (int j = tid; j < s_used; j += stride) {
     const int b = last_at_most(s_page, B, j);
-    const int have = (s_cached[b] + page - 1) / page;
+    const int have = pages_of(s_cached[b], page);
     p.tables[b * p.table_stride + have + j - s_page[b]] = p.free_pages[free_count - 1 - j];
   }
   // tokens: one a thread while that is enough, else 4 neighbours, with one search and their reads
@@ -277,7 +283,7 @@ __global__ void __launch_bounds__(kReleaseThreads)
       if (threadIdx.x == 0) record_error(err, LM_DEVERR_BAD_LENGTH);
       continue;  // the same decision in every thread: nothing of the row changes
     }
-    const int n = (cached[b] + page_size - 1) / page_size;
+    const int n = pages_of(cached[b], page_size);
     int32_t* row = tables + b * table_stride;
     if (n > free_capacity - count) {
       int pages = 0;
