@@ -128,3 +128,17 @@ def test_refusals(cuda):
         dec.generate([[1], [2], []], 4, 8)
     with pytest.raises(ValueError):
         dec.generate([[1], [2], [3]], 4, 199)
+
+
+def test_tokens_outside_the_vocabulary_are_refused(cuda):
+    """Before anything is launched: the embedding's rows are read at the tokens' numbers."""
+    dec = _make(cuda)
+    for bad in ([TINY.vocab], [3, -1], [-(2 ** 31)], [2 ** 40]):
+        with pytest.raises(ValueError, match="token"):
+            dec.step([[1, 2], bad, ()])
+        with pytest.raises(ValueError, match="token"):
+            dec.generate([[1, 2], bad, [5]], 4, 64)
+    assert dec.cache.lens.tolist() == [0, 0, 0]
+    dec.step([[0, TINY.vocab - 1], None, ()])
+    dec.cache.check_errors()
+    assert dec.cache.lens.tolist() == [2, 1, 0]

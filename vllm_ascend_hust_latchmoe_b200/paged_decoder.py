@@ -181,10 +181,17 @@ class PagedMoEDecoder:
         torch.mm(h.index_select(0, last), self.lm_head.t(), out=self.logits)
         self.next_token.copy_(self.logits.argmax(-1))
 
+    def _check_tokens(self, rows: Sequence[Sequence[int] | None]) -> None:
+        """The embedding's rows are read at these numbers."""
+        for r in rows:
+            if r is not None and len(r) and not 0 <= min(r) <= max(r) < self.s.vocab:
+                raise ValueError(f"a token outside 0 .. {self.s.vocab - 1}")
+
     def step(self, rows: Sequence[Sequence[int] | None]) -> None:
         """One step: ``rows[b]`` is row b's next prompt chunk, or None for the token that the last
         step gave it, or () for nothing. Afterwards ``logits`` and ``next_token`` hold every row's
         (rows without new tokens: undefined)."""
+        self._check_tokens(rows)
         new = [1 if r is None else len(r) for r in rows]
         T = self.cache.set_new_lens(new)
         if T == 0:
@@ -218,6 +225,7 @@ class PagedMoEDecoder:
         the rows that decode already."""
         if len(prompts) != self.max_requests or any(len(p) == 0 for p in prompts):
             raise ValueError(f"{self.max_requests} prompts of at least a token are wanted")
+        self._check_tokens(prompts)
         if chunk < 1 or chunk + self.max_requests > self.max_tokens:
             raise ValueError("chunk + requests must fit a step's tokens")
         taken, made = [0] * len(prompts), [0] * len(prompts)
