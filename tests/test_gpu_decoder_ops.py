@@ -860,3 +860,28 @@ def test_page_tables_pages_near_2_31_tokens(cuda):
     tables, lens, free, count = (torch.tensor(v, **one) for v in ([[3]], [2 ** 31 - 2], [-8, -8], [0]))
     ops.release_pages(torch.zeros(1, **one), lens, 2 ** 31 - 1, tables, free, count)
     assert free.tolist() == [3, -8] and count.item() == 1 and lens.item() == 0 and tables.item() == -1
+
+
+def test_strides_of_dimensions_of_one_do_not_count(cuda):
+    """One token out of a wider row, or one head: nothing is read at that stride, whatever it says."""
+    g = _gen(cuda, 31)
+    D, Hq = 64, 4
+    ws = ops.attention_workspace(cuda)
+    i32 = dict(dtype=torch.int32, device=cuda)
+    cs = torch.cat([torch.ones(8, D, device=cuda)[:, :32], torch.zeros(8, 32, device=cuda)], 1)
+    for Hkv in (1, 2):
+        kc, vc = _bf16(g, 3, 16, Hkv, D), _bf16(g, 3, 16, Hkv, D)
+        if Hkv == 1:
+            kc, vc = (c.as_strided(c.shape, (16 * D, D, 3, 1)) for c in (kc, vc))
+        qkv = _bf16(g, 1, (Hq + 2 * Hkv) * D)
+        qkv = qkv.as_strided(qkv.shape, ((Hq + 2 * Hkv) * D + 5, 1))
+        q, out = (_bf16(g, 1, Hq, D).as_strided((1, Hq, D), (7, D, 1)) for _ in range(2))
+        ops.rope_cache_write(qkv, torch.zeros(1, **i32), torch.tensor([40], device=cuda), cs, kc, vc, q)
+        x = qkv.view(Hq + 2 * Hkv, D)
+        assert torch.equal(q[0], x[:Hq]) and torch.equal(kc[2, 8], x[Hq:Hq + Hkv])
+        assert torch.equal(vc[2, 8], x[Hq + Hkv:])
+        tables = torch.tensor([[1, 0, 2]], **i32)
+        ops.paged_attention(q, kc, vc, tables, torch.tensor([41], **i32), torch.tensor([0, 1], **i32), out,
+                            max_q_len=1, workspace=ws)
+        want, _, tol, _ = _attention64(q, kc, vc, tables, [41], [0, 1], D ** -0.5, 0)
+        _within(out, want, tol)

@@ -109,6 +109,12 @@ class Check {
   int64_t device_ = -1;
 };
 
+// A dimension of one has no stride of its own (torch keeps whatever the tensor was cut from); the C ABI
+// takes multiples of 8, so such a one passes as `of_one`.
+int64_t stride(const Tensor& t, int64_t dim, int64_t of_one = 0) {
+  return t.size(dim) == 1 ? of_one : t.stride(dim);
+}
+
 uint16_t* bits(const Tensor& t) { return static_cast<uint16_t*>(t.data_ptr()); }
 uint16_t* bits(const OptTensor& t) { return t ? bits(*t) : nullptr; }
 int32_t* ints(const Tensor& t) { return static_cast<int32_t*>(t.data_ptr()); }
@@ -217,13 +223,13 @@ void rope_cache_write(const Tensor& qkv, const Tensor& positions, const Tensor& 
   if (q_weight) c.dense("q_norm_weight", *q_weight, at::kBFloat16, {D});
   if (k_weight) c.dense("k_norm_weight", *k_weight, at::kBFloat16, {D});
   done("lm_rope_cache_write",
-       lib.rope_cache_write(bits(qkv), qs, ints(positions), static_cast<const int64_t*>(slots.data_ptr()), T,
+       lib.rope_cache_write(bits(qkv), T == 1 ? 0 : qs, ints(positions), static_cast<const int64_t*>(slots.data_ptr()), T,
                             narrow("heads", Hq), narrow("heads", Hkv), narrow("head_dim", D),
                             static_cast<const float*>(cos_sin.data_ptr()), narrow("cos_sin", cos_sin.size(0)),
                             narrow("cos_sin", cos_sin.size(1)), interleaved ? 1 : 0, bits(q_weight),
-                            bits(k_weight), static_cast<float>(eps), bits(q_out), q_out.stride(0),
-                            q_out.stride(1), bits(k), k.stride(0), k.stride(1), k.stride(2), bits(v),
-                            v.stride(0), v.stride(1), v.stride(2), k.size(0), narrow("page_size", k.size(1)),
+                            bits(k_weight), static_cast<float>(eps), bits(q_out), stride(q_out, 0),
+                            stride(q_out, 1), bits(k), stride(k, 0), stride(k, 1), stride(k, 2), bits(v),
+                            stride(v, 0), stride(v, 1), stride(v, 2), k.size(0), narrow("page_size", k.size(1)),
                             c.err(err_word), c.stream()));
 }
 
@@ -244,14 +250,14 @@ void paged_attention(const Tensor& q, const Tensor& k, const Tensor& v, const Te
   c.dense("workspace", workspace, at::kByte, {-1});
   if (lse) c.dense("lse", *lse, at::kFloat, {T, Hq});
   done("lm_paged_attention",
-       lib.paged_attention(bits(q), q.stride(0), q.stride(1), bits(k), k.stride(0), k.stride(1), k.stride(2),
-                           bits(v), v.stride(0), v.stride(1), v.stride(2), k.size(0),
+       lib.paged_attention(bits(q), stride(q, 0), stride(q, 1), bits(k), stride(k, 0), stride(k, 1),
+                           stride(k, 2, D), bits(v), stride(v, 0), stride(v, 1), stride(v, 2, D), k.size(0),
                            narrow("page_size", k.size(1)), ints(tables), ts,
                            narrow("block_tables", tables.size(1)), ints(seq_lens), ints(cu_q),
                            narrow("requests", B), T, narrow("heads", Hq), narrow("heads", k.size(2)),
                            narrow("head_dim", D), narrow("max_q_len", max_q_len),
                            static_cast<float>(scale ? *scale : 1.0 / std::sqrt(static_cast<double>(D))),
-                           narrow("window", window), bits(out), out.stride(0), out.stride(1),
+                           narrow("window", window), bits(out), stride(out, 0), stride(out, 1),
                            lse ? static_cast<float*>(lse->data_ptr()) : nullptr, workspace.data_ptr(),
                            workspace.numel(), c.err(err_word), c.stream()));
 }
