@@ -885,3 +885,43 @@ def test_strides_of_dimensions_of_one_do_not_count(cuda):
                             max_q_len=1, workspace=ws)
         want, _, tol, _ = _attention64(q, kc, vc, tables, [41], [0, 1], D ** -0.5, 0)
         _within(out, want, tol)
+
+
+def test_attention_first_called_from_several_host_threads(cuda):
+    """Through the C ABI (ctypes leaves the interpreter's lock), in a process that has not called it yet: each
+    thread on a stream and a workspace of its own."""
+    code = """
+import ctypes, threading, torch
+import tests.test_gpu_decoder_ops as t
+from vllm_ascend_hust_latchmoe_b200 import _lib
+dev, lib, P = torch.device('cuda', 0), _lib.load(), ctypes.c_void_p
+g = t._gen(dev, 3)
+kc, vc = t._bf16(g, 40, 16, 2, 64), t._bf16(g, 40, 16, 2, 64)
+ids = torch.arange(40, dtype=torch.int32, device=dev).view(1, 40)
+sizes = [(1, 300), (70, 600), (3, 640), (200, 200)] * 2
+cases = []
+for n, L in sizes:
+    q = t._bf16(g, n, 8, 64)
+    cases.append((q, torch.empty_like(q), torch.tensor([L], dtype=torch.int32, device=dev),
+                  torch.tensor([0, n], dtype=torch.int32, device=dev), torch.zeros(1, dtype=torch.int32, device=dev),
+                  torch.zeros(200 << 20, dtype=torch.uint8, device=dev), torch.cuda.Stream()))
+torch.cuda.synchronize()
+gate, rcs = threading.Barrier(len(cases)), []
+def work(q, out, seq, cu, err, ws, stream):
+    p = [P(x.data_ptr()) for x in (q, kc, vc, ids, seq, cu, out, ws, err)]
+    gate.wait()
+    rc = lib.lm_paged_attention(p[0], 512, 64, p[1], 2048, 128, 64, p[2], 2048, 128, 64, 40, 16, p[3], 40, 40,
+                                p[4], p[5], 1, q.shape[0], 8, 2, 64, q.shape[0], 0.125, 0, p[6], 512, 64, None, p[7],
+                                ws.numel(), p[8], P(stream.cuda_stream))
+    rcs.append((rc, rc and lib.lm_last_error()))
+threads = [threading.Thread(target=work, args=c) for c in cases]
+[x.start() for x in threads]
+[x.join() for x in threads]
+torch.cuda.synchronize()
+assert rcs == [(0, 0)] * len(cases), rcs
+for (q, out, *_), (n, L) in zip(cases, sizes):
+    want, _, tol, _ = t._attention64(q, kc, vc, ids, [L], [0, n], 0.125, 0)
+    t._within(out, want, tol)
+"""
+    done = subprocess.run([sys.executable, "-c", code], cwd=ROOT, capture_output=True, text=True, timeout=300)
+    assert done.returncode == 0, done.stderr[-2000:]

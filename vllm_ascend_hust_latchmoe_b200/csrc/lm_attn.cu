@@ -12,7 +12,6 @@
 // they read last) at the end of a segment. Segments of an item that several CTAs share are merged
 // through the workspace, by the CTA that arrives last, in the order of the keys.
 #include <algorithm>
-#include <string>
 
 #include "lm_attn.cuh"
 #include "lm_attn_ring.cuh"
@@ -458,8 +457,6 @@ struct Workspace {
 // one head x 64 values.
 int cache_map(CUtensorMap* out, const void* base, const AttnParams& a, int head_dim, int64_t page_stride,
               int64_t token_stride, int64_t head_stride, int box_rows, bool heads_first) {
-  auto fn = tensor_map_encode_fn();
-  if (fn == nullptr) return fail(LM_ERR_CUDA, "cuTensorMapEncodeTiled is unavailable");
   // a dimension of one has no stride of its own
   if (a.kv_heads == 1) head_stride = head_dim;
   if (a.num_pages == 1) page_stride = std::max(token_stride, head_stride);
@@ -474,14 +471,7 @@ int cache_map(CUtensorMap* out, const void* base, const AttnParams& a, int head_
   strides[t - 1] = static_cast<cuuint64_t>(token_stride) * 2;
   strides[2] = static_cast<cuuint64_t>(page_stride) * 2;
   box[t] = static_cast<cuuint32_t>(box_rows);
-  const cuuint32_t unit[4] = {1, 1, 1, 1};
-  const CUresult r = fn(out, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 4, const_cast<void*>(base), dims, strides,
-                        box, unit, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
-                        CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
-  if (r != CUDA_SUCCESS)
-    return fail(LM_ERR_CUDA, "lm_paged_attention: cuTensorMapEncodeTiled failed with CUresult " +
-                                 std::to_string(r));
-  return LM_OK;
+  return encode_bf16_map(out, 4, base, dims, strides, box);
 }
 
 template <int D>

@@ -49,7 +49,26 @@ MapCache& map_cache() {
 
 }  // namespace
 
-PFN_cuTensorMapEncodeTiled_v12000 tensor_map_encode_fn() { return encode_fn(); }
+int encode_bf16_map(CUtensorMap* out, int rank, const void* ptr, const cuuint64_t* dims,
+                    const cuuint64_t* strides, const cuuint32_t* box) {
+  auto fn = encode_fn();
+  if (fn == nullptr) return fail(LM_ERR_CUDA, "cuTensorMapEncodeTiled is unavailable");
+  const cuuint32_t unit[5] = {1, 1, 1, 1, 1};
+  auto encode = [&] {
+    return fn(out, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, static_cast<cuuint32_t>(rank), const_cast<void*>(ptr), dims,
+              strides, box, unit, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+              CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  };
+  CUresult r = encode();
+  int dev = 0;
+  // A host thread that has made no runtime call yet has no current context, which this driver call wants;
+  // cudaSetDevice binds the device's own (and, unlike an allocation, may stand inside a stream capture).
+  if (r == CUDA_ERROR_INVALID_CONTEXT && cudaGetDevice(&dev) == cudaSuccess && cudaSetDevice(dev) == cudaSuccess)
+    r = encode();
+  if (r != CUDA_SUCCESS)
+    return fail(LM_ERR_CUDA, "cuTensorMapEncodeTiled failed with CUresult " + std::to_string(r));
+  return LM_OK;
+}
 
 int make_map(CUtensorMap* out, const void* ptr, int rank, uint64_t d0, uint64_t d1,
              int box_rows, int box_depth) {
@@ -63,8 +82,6 @@ int make_map(CUtensorMap* out, const void* ptr, int rank, uint64_t d0, uint64_t 
         return LM_OK;
       }
   }
-  auto fn = encode_fn();
-  if (fn == nullptr) return fail(LM_ERR_CUDA, "cuTensorMapEncodeTiled is unavailable");
   cuuint64_t dims[3];
   cuuint64_t strides[2];
   if (rank == 2) {
@@ -80,14 +97,9 @@ int make_map(CUtensorMap* out, const void* ptr, int rank, uint64_t d0, uint64_t 
   }
   cuuint32_t box[3] = {static_cast<cuuint32_t>(BK), static_cast<cuuint32_t>(box_rows),
                        static_cast<cuuint32_t>(box_depth)};
-  cuuint32_t estr[3] = {1, 1, 1};
   CUtensorMap m;
-  const CUresult r = fn(&m, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, static_cast<cuuint32_t>(rank),
-                        const_cast<void*>(ptr), dims, strides, box, estr,
-                        CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
-                        CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
-  if (r != CUDA_SUCCESS)
-    return fail(LM_ERR_CUDA, "cuTensorMapEncodeTiled failed with CUresult " + std::to_string(r));
+  const int rc = encode_bf16_map(&m, rank, ptr, dims, strides, box);
+  if (rc) return rc;
   {
     std::lock_guard<std::mutex> lk(cache.mu);
     if (cache.entries.size() >= 256) cache.entries.erase(cache.entries.begin());

@@ -17,7 +17,8 @@ namespace lm {
 int make_map(CUtensorMap* out, const void* ptr, int rank, uint64_t d0, uint64_t d1,
              int box_rows = 128, int box_depth = 1);
 
-// The driver's cuTensorMapEncodeTiled, for maps of other shapes (null if there is none).
-PFN_cuTensorMapEncodeTiled_v12000 tensor_map_encode_fn();
+// Map of any rank over bf16 values: 128-byte swizzle, zeros out of range; `strides` in bytes.
+int encode_bf16_map(CUtensorMap* out, int rank, const void* ptr, const cuuint64_t* dims,
+                    const cuuint64_t* strides, const cuuint32_t* box);
 
 }  // namespace lm
