@@ -12,6 +12,7 @@
 // they read last) at the end of a segment. Segments of an item that several CTAs share are merged
 // through the workspace, by the CTA that arrives last, in the order of the keys.
 #include <algorithm>
+#include <atomic>
 
 #include "lm_attn.cuh"
 #include "lm_attn_ring.cuh"
@@ -427,15 +428,17 @@ __global__ void __launch_bounds__(kThreads, 1)
 }
 
 int attn_ctas() {
-  static int cached[64] = {0};
+  static std::atomic<int> cached[64];
   int dev = 0;
   if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return 148;
-  if (cached[dev] == 0) {
-    int n = 148;
+  int n = cached[dev].load(std::memory_order_relaxed);
+  if (n == 0) {
+    n = 148;
     cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev);
-    cached[dev] = n < kAttnMaxCtas ? n : kAttnMaxCtas;
+    n = n < kAttnMaxCtas ? n : kAttnMaxCtas;
+    cached[dev].store(n, std::memory_order_relaxed);
   }
-  return cached[dev];
+  return n;
 }
 
 // The workspace: for either kernel its counters, and the sums and accumulators of 2 partial results
@@ -482,17 +485,17 @@ int launch_rows(const AttnParams& a, const AttnMaps& maps, bool beside, cudaStre
   p.negate_q = 0;
   p.beside = beside;
   const size_t smem = RowsSmem<D>::kBytes + (static_cast<size_t>(a.num_requests) + 1) * 4;
-  static bool done[64] = {false};
+  static std::atomic<bool> done[64];  // two threads may both set the attribute, to the same value
   int dev = 0;
   cudaGetDevice(&dev);
   if (dev < 0 || dev >= 64) return fail(LM_ERR_UNSUPPORTED, "lm_paged_attention: device index >= 64");
-  if (!done[dev]) {
+  if (!done[dev].load(std::memory_order_acquire)) {
     const int rc = check_cuda(
         cudaFuncSetAttribute(paged_attn_rows_kernel<D>, cudaFuncAttributeMaxDynamicSharedMemorySize,
                              RowsSmem<D>::kBytes + (kAttnMaxRequests + 1) * 4),
         "lm_paged_attention: smem attribute");
     if (rc) return rc;
-    done[dev] = true;
+    done[dev].store(true, std::memory_order_release);
   }
   return check_cuda(launch_dependent(paged_attn_rows_kernel<D>, dim3(attn_ctas()), dim3(kThreads),
                                      smem, s, p),

@@ -27,6 +27,8 @@
 // exponent bits), 2^100 of range is left for V and the number of keys, and the division by the sum
 // at the end takes the reference out again. A move costs its stream some 700 cycles, and with a
 // bound of 2^8 sharp heads moved one of 128 rows in most blocks.
+#include <atomic>
+
 #include "lm_attn.cuh"
 
 namespace lm {
@@ -644,11 +646,11 @@ __global__ void __launch_bounds__(kThreads, 1)
 
 template <int D>
 int launch(const AttnLaunch& p, int ctas, cudaStream_t s) {
-  static bool done[64] = {false};
+  static std::atomic<bool> done[64];  // two threads may both set the attribute, to the same value
   int dev = 0;
   cudaGetDevice(&dev);
   if (dev < 0 || dev >= 64) return fail(LM_ERR_UNSUPPORTED, "lm_paged_attention: device index >= 64");
-  if (!done[dev]) {
+  if (!done[dev].load(std::memory_order_acquire)) {
     // setmaxnreg hands out the registers that the CTA was launched with, and waits for ones that it
     // does not have
     cudaFuncAttributes attr;
@@ -660,7 +662,7 @@ int launch(const AttnLaunch& p, int ctas, cudaStream_t s) {
                                            cudaFuncAttributeMaxDynamicSharedMemorySize, UmmaCfg<D>::kSmem),
                       "lm_paged_attention: smem attribute");
     if (rc) return rc;
-    done[dev] = true;
+    done[dev].store(true, std::memory_order_release);
   }
   return check_cuda(launch_dependent(paged_attn_umma_kernel<D>, dim3(ctas), dim3(kThreads),
                                      UmmaCfg<D>::kSmem, s, p),
