@@ -265,6 +265,7 @@ void paged_attention(const Tensor& q, const Tensor& k, const Tensor& v, const Te
 }  // namespace
 
 PYBIND11_MODULE(_decoder_ops, m) {
+  m.attr("built_for") = LM_BUILT_FOR;
   m.def("bind", &bind);
   m.def("add_rms_norm", &add_rms_norm);
   m.def("build_page_tables", &build_page_tables);

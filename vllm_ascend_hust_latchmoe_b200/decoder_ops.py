@@ -23,7 +23,7 @@ import importlib.util
 import torch
 
 from . import _lib
-from ._build import BINDING_PATH
+from ._build import BINDING_PATH, binding_key
 
 _binding = None
 
@@ -39,6 +39,9 @@ def _load():
     spec = importlib.util.spec_from_file_location("_decoder_ops", BINDING_PATH)
     module = importlib.util.module_from_spec(spec)
     spec.loader.exec_module(module)
+    if module.built_for != binding_key():
+        raise RuntimeError(f"{BINDING_PATH} was built for {module.built_for}, this is {binding_key()}: "
+                           "build it again")
     lib = _lib.lib()
     for name in ("lm_last_error", "lm_add_rms_norm", "lm_build_page_tables", "lm_release_pages",
                  "lm_rope_cache_write", "lm_paged_attention"):
