@@ -110,7 +110,8 @@ __device__ __forceinline__ void place_tokens(const TableParams& p, const int32_t
       const int kept = s_cached[lo], c = kept < 0 ? ~kept : kept;
       pos[e] = c + static_cast<int>(t) - s_cu[lo];
       if (kept < 0) continue;
-      const int have = pages_of(c, page), i = pos[e] / page;
+      const int have = pages_of(c, page);  // unsigned like the next line, which shares its divisor's set-up
+      const int i = static_cast<int>(static_cast<uint32_t>(pos[e]) / static_cast<uint32_t>(page));
       // pages already held are read from the table, granted ones from the stack (another CTA may be
       // writing their table entries)
       const int id = i < have ? p.tables[lo * p.table_stride + i]
