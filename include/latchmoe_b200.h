@@ -490,7 +490,7 @@ int lm_ep_combine(const int32_t* topk_ids, const uint16_t* topk_weights_bf16,
  * y = z * rsqrt(mean(z^2) + eps) * weight, rounded once to bf16 (y) or to e4m3 (y8, with fp32
  * scales: s = max(max|y|, 1e-12) / 448 per row (group_size 0, scales [T]) or per group_size
  * columns (a multiple of 32 that divides hidden_size; scales [T][hidden_size / group_size]);
- * y8 = e4m3(y / s)). Exactly one of y and y8. residual and residual_out may be NULL;
+ * y8 = e4m3(y / s), the fp32 quotient within 3 units of its last place). Exactly one of y and y8. residual and residual_out may be NULL;
  * residual_out may be residual or x itself (with the same stride), other overlaps may not.
  * Strides are row strides in elements; hidden_size <= 16384. */
 int lm_add_rms_norm(const uint16_t* x, int64_t x_stride, const uint16_t* residual,

@@ -611,8 +611,9 @@ extern "C" int lm_paged_attention(
   // rows go to the tensor-core kernel. A call with both kinds makes both launches, unless its short
   // requests can only be a little work (by the block table's width, all of them single tokens): the
   // tensor-core kernel takes 1.9 us for a block of keys and the row kernel 1.4, but a second launch
-  // costs 3 to 5 us (a 512-token chunk beside 7 single tokens over 4000 keys: 49 against 59 us in two
-  // launches, beside 15 of them 65 against 70).
+  // costs 3 to 6 us (a 512-token chunk beside 7 single tokens over 4000 keys, 32 heads on 4: 36 us in
+  // one launch and 42 in two, beside 15 of them 42 and 45). The lengths are on the device and the width is
+  // what the host knows, so a call with much wider tables than its requests fill takes two launches.
   const bool any_long = static_cast<int64_t>(max_q_len) * p.group > kTileRows;
   const int64_t short_units = static_cast<int64_t>(num_requests) * num_kv_heads *
                               ((static_cast<int64_t>(max_pages) * page_size + kBlock - 1) / kBlock);

@@ -12,9 +12,11 @@
 // The weights are rounded to bf16 as the MMA's operand (the error of an output then has sqrt(2) times
 // the rms of its own rounding); their sum takes them unrounded.
 //
-// Measured: a 4096-token chunk over 16384 keys, 32 / 4 heads of 128: 737 to 760 us in short graph
-// replays (1265 to 1305 TFLOP/s, 74 to 77 % of the burst GEMM rate), 862 us in stretches of seconds
-// under the power cap (1117 TFLOP/s, 78 % of the sustained rate). A block pair takes some 3500 cycles: 2300 from S to P
+// Measured: a 4096-token chunk over 16384 keys, 32 / 4 heads of 128: 731 to 760 us in short graph
+// replays (1265 to 1316 TFLOP/s, 74 to 77 % of the burst GEMM rate), 850 to 875 us in stretches of seconds
+// under the power cap (1100 to 1130 TFLOP/s, 77 to 80 % of the sustained rate). With heads of 64: 588 to
+// 603 us, 800 TFLOP/s; at 16 exponentials a clock and SM its 1.9e9 of them take some 420 us, its MMAs
+// 283 us at the burst rate. With heads of 128, a block pair takes some 3500 cycles: 2300 from S to P
 // (read 160, maximum 400, exponentials 2 x 740) and 1200 from P to the next S, against 2048 of MMAs.
 // Tried without gain: part of the exponentials on the FMA pipe (782 - 852 us for 1/8 to 1/2 of them),
 // the first exponentials beside the maximum (884 us), the next item's Q begun ahead of its
@@ -447,7 +449,8 @@ __global__ void __launch_bounds__(kThreads, 1)
           }
           const int j0 = blk * kBlk;
           // 32 keys at a time, so that a block on the diagonal is not all compared (8 prompts of 1024
-          // tokens, 64 heads on 4: 248 -> 232 us; windows of 512 keys 151 -> 140 us)
+          // tokens, 64 heads on 4: 248 -> 232 us; a window of 512 keys, 4 requests of 2000 new tokens over
+          // 2000, 32 heads on 4 of 128: 151 -> 140 us, floor 39)
           if (j0 + kBlk - 1 > high_min || j0 <= low_max) {
 #pragma unroll
             for (int i = 0; i < 4; ++i) {

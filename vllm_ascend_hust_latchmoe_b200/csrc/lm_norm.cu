@@ -1,7 +1,8 @@
 // Residual addition + RMS norm of a decoder layer, with a bf16 or an e4m3 + scales output:
 //   z = x + residual;  y = z * rsqrt(mean(z^2) + eps) * weight
 //   e4m3: per group (a whole row, or group_size columns) s = max(max|y|, 1e-12) / 448,
-//         y8 = e4m3(y / s)
+//         y8 = e4m3(y / s), the quotient in fp32 as a product with 1 / s: within 3 units of its last
+//         place, so that a value next to the middle of two e4m3 values may take the other one
 // z, the sum of squares and the scales are fp32; z is rounded to bf16 once for residual_out and
 // is normalised unrounded, y is rounded once to its output type.
 #include <atomic>
@@ -96,8 +97,9 @@ __device__ __forceinline__ float block_reduce(float v, float* s_red) {
 // values a thread, piece i of thread t at column (i * blockDim + t) * VEC), the weight is loaded
 // once, and the next row's loads are issued before this row's sums are joined. HBM-bound: measured
 // 6.4 TB/s (99 % of the copy rate) at 16384 x 4096 with e4m3 output, 6.0 TB/s with bf16 output;
-// 12.1 us at 4093 x 2048 (5.5 TB/s) and 1.5 us a call at 16 x 2048, both replayed from a graph. Rows
-// that no 16-byte load fits (VEC 1) run at 3.8 TB/s with bf16 output and 2.0 with e4m3.
+// 12.1 to 12.8 us at 4093 x 2048 (5.2 to 5.5 TB/s) and 1.5 us a call at 16 x 2048, both replayed from a
+// graph. Rows that no 16-byte load fits (VEC 1, with 2-byte loads and 2- or 1-byte stores) run at 4.1 TB/s
+// with bf16 output and 2.0 with e4m3 (16384 x 4095; 4096 x 1001: 10.4 and 17.4 us).
 template <int VEC, int VPT, bool FP8>
 __global__ void __launch_bounds__(VEC == 8 ? 256 : 1024)
     add_rms_norm_kernel(const NormParams p) {

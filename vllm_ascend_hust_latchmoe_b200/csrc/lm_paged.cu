@@ -139,7 +139,7 @@ __device__ __forceinline__ void place_tokens(const TableParams& p, const int32_t
 // Every CTA scans all requests (they fit one pass of its threads) and writes its share of the
 // tables and of the tokens. All reads of arrays that the call may overwrite in place (cached
 // lengths, the free count) come before the cluster's barrier, all writes to them after it.
-// Latency-bound: 4.2 us a call for 64 requests with a token each, 8.9 us for 1021 requests with 30,000
+// Latency-bound: 4.2 us a call for 64 requests with a token each, 8.8 us for 1021 requests with 30,000
 // tokens (replayed from a graph; 20.6 us when a request's pages were one warp's).
 __global__ void __launch_bounds__(kTableThreads) page_tables_kernel(const TableParams p) {
   pdl_wait();
@@ -259,8 +259,9 @@ __global__ void __launch_bounds__(kTableThreads) page_tables_kernel(const TableP
 // One block: the pages of the listed rows go back onto the free stack in row order. Entries below 0 hold
 // no page (it was given back before, as behind a sliding window) and are passed over; where a row's
 // entries are more than the stack has room for, its pages are counted first, so that a row whose pages do
-// not fit stays as it is. The rows follow one another, each a chain of dependent reads: 6.2 us a call for
-// one row of 80 pages, 14 us for 16, 335 us for 512 (pushed unchecked they took 279 us).
+// not fit stays as it is. The rows follow one another, each a chain of dependent reads: 6 to 7 us a call
+// for one row of 80 pages, 14 us for 16 such rows, 320 to 335 us for 512 (265 to 279 us when entries were
+// pushed unchecked).
 constexpr int kReleaseThreads = 256;
 
 __global__ void __launch_bounds__(kReleaseThreads)
@@ -376,8 +377,10 @@ __device__ __forceinline__ int rope_position(const RopeParams& p, int pos) {
 // heads' loads are in flight together. A lane's partners are its own neighbours (interleaved) or
 // the 8 values of the lane half / 8 away, which come by shuffle as the bf16 pairs they are. Needs
 // 8 | rot_dim, and 16 | rot_dim for pairs half a rotation apart. Measured at 4096 tokens x 40 heads
-// of 128 with norms: 18.5 us (4.6 TB/s, 72 % of the copy rate); instruction issue bounds it more
-// than memory does (a version with 213 instructions per 32 lanes took 26.6 us, one with 156 21.5 us).
+// of 128 with norms: 18.2 to 18.6 us (4.6 TB/s, 72 % of the copy rate). Neither limit is reached: issue
+// slots are 67 % busy (a version with 213 instructions per 32 lanes took 26.6 us, one with 156 21.5 us)
+// and DRAM moves 2.5 TB/s, since most writes stay in L2. The blocks are uneven: 1536 of them at 4 an SM
+// make 2.6 waves, and one of queries does eight times the work of one of K or V.
 // With one group of heads a warp, 2 or 8 heads in flight per lane measured 24.7 and 21.7 us in the
 // place of 21.5, more registers or more blocks per SM 23.7 and 26.7 us; the next group's loads ahead of
 // this one's arithmetic spill (20.6 us). 16 tokens take 3.2 us.
@@ -396,8 +399,13 @@ __host__ __device__ constexpr int rope_heads_per_warp() {
 }
 
 // Q chunks that a warp takes one after the other, with the rotation and weight in registers. Many
-// tokens fill the GPU anyway (4096 x 40 heads: 18.5 us with 4 against 21.5 with 1); few tokens wait
-// for one warp's chain (16: 6.8 against 3.2 us).
+// tokens fill the GPU anyway; few tokens wait for one warp's chain. With 4 against 1, in us:
+//   tokens                  64          1024          1536          2048          3000          4096
+//   64/4 heads of 128   6.8, 3.2     13.5, 11.4   15.5, 15.5   16.9, 19.5   25.1, 26.8   30.0, 35.0
+//   32/4 heads of 128   6.8, 3.2     10.2, 7.2    13.0, 9.9    13.6, 12.9   15.9, 17.0   18.6, 21.6
+//   16/2 heads of 128   4.7, 3.2      5.7, 4.7     6.4, 5.2     7.9, 7.0    10.3, 10.8   12.9, 13.9
+//   32/8 heads of 64    4.2, 3.1      5.7, 4.7     6.7, 5.7     8.6, 8.3    10.5, 11.3   13.4, 14.4
+// They cross between 1536 and 3000 tokens, the earlier the more query heads there are.
 constexpr int kRopeLoops = 4;
 constexpr int64_t kRopeManyTokens = 2048;
 
@@ -548,7 +556,9 @@ __global__ void __launch_bounds__(kRopeWarps * 32, 4) rope_write_kernel(const Ro
 }
 
 // Any even rot_dim: a warp per (token, head); the head's fp32 values pass through shared memory so
-// that a lane reads its rotation partner.
+// that a lane reads its rotation partner. 2-byte accesses, and the token's rotation and a 64-bit division
+// again for every head: 47 us at 4096 tokens x 40 heads of 128 with rot_dim 30, 56 us with 120, where
+// the other kernel takes 18.5 us. For sizes that models rarely have.
 template <int D>
 __global__ void __launch_bounds__(kRopeWarps * 32) rope_write_any_kernel(const RopeParams p) {
   pdl_wait();
@@ -716,7 +726,7 @@ extern "C" int lm_rope_cache_write(
                      v_head_stride, num_tokens, num_pages * page_size, eps, num_q_heads,
                      num_kv_heads, rot_dim, max_positions, page_size, interleaved};
   // Pieces of 8 values where the rotation is made of them, else (an odd rot_dim, a table or weights
-  // that no 16-byte load fits) a warp per head: 18.5 against 52 us at 4096 tokens x 40 heads of 128.
+  // that no 16-byte load fits) a warp per head: 18.5 against 47 to 56 us at 4096 tokens x 40 heads of 128.
   const bool wide = rot_dim % (interleaved ? 8 : 16) == 0 &&
                     ((reinterpret_cast<uintptr_t>(cos_sin) | reinterpret_cast<uintptr_t>(q_norm_weight) |
                       reinterpret_cast<uintptr_t>(k_norm_weight)) & 15) == 0;

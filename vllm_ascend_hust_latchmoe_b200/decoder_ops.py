@@ -58,7 +58,8 @@ def add_rms_norm(x: torch.Tensor, weight: torch.Tensor, eps: float = 1e-6, *,
     """``z = x + residual``; ``residual_out = bf16(z)``;
     ``y = z * rsqrt(mean(z^2) + eps) * weight`` into ``out`` (bf16 ``[T, H]``) or ``out_fp8``
     (e4m3 ``[T, H]``) with fp32 ``scales`` ``[T, 1]`` (``group_size`` 0) or
-    ``[T, H / group_size]``: ``scale = max(max|y|, 1e-12) / 448``, ``out_fp8 = e4m3(y / scale)``.
+    ``[T, H / group_size]``: ``scale = max(max|y|, 1e-12) / 448``, ``out_fp8 = e4m3(y / scale)`` (the
+    fp32 quotient within 3 units of its last place).
 
     ``x`` ``[T, H]`` and the other rows may have any row stride; ``residual_out`` may be
     ``residual`` or ``x`` (in place). ``H`` is at most 16384."""
